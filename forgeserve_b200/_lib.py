@@ -36,6 +36,18 @@ class KVCacheDesc(ctypes.Structure):
     ]
 
 
+class KVQuantDesc(ctypes.Structure):
+    """Mirror of fs_kv_quant."""
+
+    _fields_ = [
+        ("cache", KVCacheDesc),
+        ("k_scale", c_vp),
+        ("v_scale", c_vp),
+        ("scale_block_stride", c_i64),
+        ("scale_head_stride", c_i64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/forgeserve_b200.h
 SIGNATURES = {
     "fs_version": (c_int, []),
@@ -67,6 +79,16 @@ SIGNATURES = {
                                     c_i64, c_i64, c_float, c_vp, c_i64, c_int, c_vp]),
     "fs_attention_decode_static": (c_int, [c_vp, c_i64, ctypes.POINTER(KVCacheDesc), c_i64, c_vp, c_vp, c_i64, c_i64,
                                            c_i64, c_i64, c_i64, c_float, c_int, c_vp]),
+    "fs_rotary_kv_write": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_int, c_vp,
+                                   ctypes.POINTER(KVCacheDesc), c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_int,
+                                   c_vp]),
+    "fs_rotary_kv_write_quant": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_int, c_vp,
+                                         ctypes.POINTER(KVQuantDesc), c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_int,
+                                         c_int, c_vp]),
+    "fs_kv_dequant": (c_int, [ctypes.POINTER(KVQuantDesc), c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_vp]),
+    "fs_attention_decode_quant_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i64]),
+    "fs_attention_decode_quant": (c_int, [c_vp, c_i64, ctypes.POINTER(KVQuantDesc), c_i64, c_vp, c_vp, c_i64, c_i64,
+                                          c_i64, c_i64, c_i64, c_float, c_vp, c_i64, c_int, c_vp]),
     "fs_embed": (c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_int, c_vp]),
     "fs_argmax": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp]),
 }

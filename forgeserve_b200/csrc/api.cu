@@ -4,6 +4,7 @@
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
+#include <mutex>
 #include <string>
 
 #include "../../include/forgeserve_b200.h"
@@ -70,9 +71,24 @@ unsigned* error_word() {
     fail("error_word: no current CUDA device");
     return nullptr;
   }
+  // One word a device, whichever thread comes first. The first call may stand inside a stream capture, where an
+  // allocation needs the relaxed mode and the word is cleared on a stream of its own (the legacy stream is closed to
+  // captures).
+  static std::mutex lock;
+  const std::lock_guard<std::mutex> hold(lock);
   if (!words[dev]) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     unsigned* p = nullptr;
-    if (cudaMalloc(&p, sizeof(unsigned)) != cudaSuccess || cudaMemset(p, 0, sizeof(unsigned)) != cudaSuccess) {
+    cudaStream_t st = nullptr;
+    const bool ok = cudaMalloc(&p, sizeof(unsigned)) == cudaSuccess &&
+                    cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess &&
+                    cudaMemsetAsync(p, 0, sizeof(unsigned), st) == cudaSuccess &&
+                    cudaStreamSynchronize(st) == cudaSuccess;
+    if (st) cudaStreamDestroy(st);
+    if (!ok && p) cudaFree(p);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) {
       fail("error_word: cudaMalloc failed");
       return nullptr;
     }
@@ -333,6 +349,113 @@ int fs_attention_decode(const void* q, int64_t ldq, const fs_kv_cache* kv, int64
   if (!err) return -1;
   return decode::launch(dtype, q, ldq, c, n_slots, positions, out, ldo, B, nh, nkv, hd, scale, splits,
                         static_cast<float*>(workspace), err, static_cast<cudaStream_t>(stream));
+}
+
+// ------------------------------------------------------------------------------------- 8-bit cache, rotary forms
+static int check_kv_quant(const fs_kv_quant* c) {
+  if (!c) return fail("kv cache descriptor is NULL");
+  if (check_kv(&c->cache)) return -1;
+  if (!c->k_scale || !c->v_scale) return fail("kv cache: NULL scales");
+  return 0;
+}
+
+static KVScales to_scales(const fs_kv_quant* c) {
+  return {c->k_scale, c->v_scale, c->scale_block_stride, c->scale_head_stride};
+}
+
+static int rotary_common(const std::string& who, const void* qkv, int64_t ld, void* q_out, int64_t ldq,
+                         const float* cos_t, const float* sin_t, int64_t rope_rows, int64_t rd, int interleaved,
+                         const int64_t* positions, const fs_kv_cache* kv, const KVScales* sc, int64_t B, int64_t T,
+                         int64_t nh, int64_t nkv, int64_t hd, int64_t slot_base, int slot_from_pos, int dtype,
+                         void* stream) {
+  if (!dtype_ok(dtype)) return fail(who + ": unsupported dtype");
+  if (B > INT32_MAX || T > INT32_MAX || B * T > INT32_MAX) return fail(who + ": too many tokens");
+  if (hd <= 0 || hd % 2 || hd > 512) return fail(who + ": head_dim must be even, 2 .. 512");
+  if (nh < 0 || nkv <= 0 || nh > 65535 || nkv > 65535) return fail(who + ": bad head counts");
+  if (rd < 0 || rd % 2 || rd > hd) return fail(who + ": rotary_dim must be even, 0 .. head_dim");
+  if (!qkv || !positions || (nh > 0 && !q_out)) return fail(who + ": NULL pointer");
+  if (rd > 0 && (!cos_t || !sin_t || rope_rows <= 0)) return fail(who + ": rotation tables missing");
+  if (ld < (nh + 2 * nkv) * hd) return fail(who + ": qkv row stride too small");
+  if (nh > 0 && ldq < nh * hd) return fail(who + ": q_out row stride too small");
+  if (!slot_from_pos && slot_base < 0) return fail(who + ": negative slot_base");
+  if (nh > 0 && !(q_out == qkv && ldq == ld)) {
+    // q_out elsewhere inside qkv would be written while other threads still read it
+    const int64_t el = dtype == F32 ? 4 : 2;
+    const char* a = static_cast<const char*>(qkv);
+    const char* b = static_cast<const char*>(q_out);
+    const int64_t na = ((B * T - 1) * ld + (nh + 2 * nkv) * hd) * el, nb = ((B * T - 1) * ldq + nh * hd) * el;
+    if (a < b + nb && b < a + na) return fail(who + ": q_out must be q's own place in qkv or lie apart from it");
+  }
+  return rotary_kv_write(dtype, qkv, ld, q_out, ldq, cos_t, sin_t, rope_rows, rd, interleaved != 0, positions,
+                         to_internal(kv), sc, B, T, nh, nkv, hd, slot_base, slot_from_pos,
+                         static_cast<cudaStream_t>(stream));
+}
+
+int fs_rotary_kv_write(const void* qkv, int64_t ld, void* q_out, int64_t ldq, const float* cos_t, const float* sin_t,
+                       int64_t rope_rows, int64_t rotary_dim, int interleaved, const int64_t* positions,
+                       const fs_kv_cache* kv, int64_t B, int64_t T, int64_t nh, int64_t nkv, int64_t hd,
+                       int64_t slot_base, int slot_from_pos, int dtype, void* stream) {
+  if (B <= 0 || T <= 0) return 0;
+  if (check_kv(kv)) return -1;
+  return rotary_common("fs_rotary_kv_write", qkv, ld, q_out, ldq, cos_t, sin_t, rope_rows, rotary_dim, interleaved,
+                       positions, kv, nullptr, B, T, nh, nkv, hd, slot_base, slot_from_pos, dtype, stream);
+}
+
+int fs_rotary_kv_write_quant(const void* qkv, int64_t ld, void* q_out, int64_t ldq, const float* cos_t,
+                             const float* sin_t, int64_t rope_rows, int64_t rotary_dim, int interleaved,
+                             const int64_t* positions, const fs_kv_quant* kv, int64_t B, int64_t T, int64_t nh,
+                             int64_t nkv, int64_t hd, int64_t slot_base, int slot_from_pos, int dtype, void* stream) {
+  if (B <= 0 || T <= 0) return 0;
+  if (check_kv_quant(kv)) return -1;
+  const KVScales sc = to_scales(kv);
+  return rotary_common("fs_rotary_kv_write_quant", qkv, ld, q_out, ldq, cos_t, sin_t, rope_rows, rotary_dim, interleaved,
+                       positions, &kv->cache, &sc, B, T, nh, nkv, hd, slot_base, slot_from_pos, dtype, stream);
+}
+
+int fs_kv_dequant(const fs_kv_quant* kv, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd, void* k_out, void* v_out,
+                  int dtype, void* stream) {
+  if (B <= 0 || n_slots <= 0) return 0;
+  if (check_kv_quant(kv)) return -1;
+  if (!dtype_ok(dtype)) return fail("fs_kv_dequant: unsupported dtype");
+  if (!k_out || !v_out) return fail("fs_kv_dequant: NULL pointer");
+  if (hd <= 0 || nkv <= 0 || hd > 65536) return fail("fs_kv_dequant: bad head_dim or head count");
+  if (B > 65535 || nkv > 65535) return fail("fs_kv_dequant: too many rows or heads");
+  if (n_slots > INT32_MAX || n_slots * hd > INT32_MAX * int64_t(128)) return fail("fs_kv_dequant: too many slots");
+  if ((n_slots - 1) / kv->cache.block_size >= kv->cache.table_cols)
+    return fail("fs_kv_dequant: the block table covers fewer slots");
+  return kv_dequant(dtype, to_internal(&kv->cache), to_scales(kv), B, n_slots, nkv, hd, k_out, v_out,
+                    static_cast<cudaStream_t>(stream));
+}
+
+int64_t fs_attention_decode_quant_workspace(int64_t B, int64_t nh, int64_t hd, int64_t n_slots) {
+  if (B <= 0 || nh <= 0 || hd <= 0 || n_slots <= 0) return 0;
+  return decode_quant::workspace_bytes(B, nh, hd, n_slots);
+}
+
+int fs_attention_decode_quant(const void* q, int64_t ldq, const fs_kv_quant* kv, int64_t n_slots,
+                              const int64_t* positions, void* out, int64_t ldo, int64_t B, int64_t nh, int64_t nkv,
+                              int64_t hd, float scale, void* workspace, int64_t workspace_bytes, int dtype,
+                              void* stream) {
+  if (B <= 0) return 0;
+  if (check_kv_quant(kv)) return -1;
+  if (!q || !positions || !out) return fail("fs_attention_decode_quant: NULL pointer");
+  if (!dtype_ok(dtype)) return fail("fs_attention_decode_quant: unsupported dtype");
+  if (n_slots <= 0) return fail("fs_attention_decode_quant: the cache view has no slots");
+  if ((n_slots - 1) / kv->cache.block_size >= kv->cache.table_cols)
+    return fail("fs_attention_decode_quant: the block table covers fewer slots");
+  if (n_slots > INT32_MAX) return fail("fs_attention_decode_quant: too many slots");
+  if (hd <= 0 || hd % 2 || hd > 256) return fail("fs_attention_decode_quant: head_dim must be even, 2 .. 256");
+  if (nkv <= 0 || nh <= 0 || nh % nkv || nh > 65535)
+    return fail("fs_attention_decode_quant: n_heads must be a multiple of n_kv_heads");
+  if (B > 65535) return fail("fs_attention_decode_quant: too many rows");
+  if (ldq < nh * hd || ldo < nh * hd) return fail("fs_attention_decode_quant: row stride too small");
+  const int64_t need = decode_quant::workspace_bytes(B, nh, hd, n_slots);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail("fs_attention_decode_quant: workspace of " + std::to_string(need) + " bytes needed");
+  if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail("fs_attention_decode_quant: the workspace must be 16-byte aligned");
+  return decode_quant::launch(dtype, q, ldq, to_internal(&kv->cache), to_scales(kv), n_slots, positions, out, ldo, B, nh,
+                              nkv, hd, scale, static_cast<float*>(workspace), static_cast<cudaStream_t>(stream));
 }
 
 int fs_embed(const int64_t* ids, int64_t n, const void* table, int64_t vocab, int64_t dim, void* out, int dtype,

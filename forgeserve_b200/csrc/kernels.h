@@ -18,6 +18,14 @@ struct KVCache {
   int64_t num_blocks;     // blocks in the cache (bounds check for table entries)
 };
 
+// The fp32 scales of an 8-bit cache: one a (slot, KV head), slots adjacent.
+struct KVScales {
+  float* k;
+  float* v;
+  int64_t block_stride;   // floats between consecutive blocks
+  int64_t head_stride;    // floats between consecutive KV heads inside a block
+};
+
 int rmsnorm(int dtype, const void* x, int64_t xs, const void* w, void* y, int64_t ys, int64_t rows, int64_t dim,
             float eps, cudaStream_t st);
 int rope_kv_write(int dtype, void* qkv, int64_t ld, const float* cos_t, const float* sin_t, int64_t rope_rows,
@@ -52,5 +60,21 @@ int launch(int dtype, const void* q, int64_t ldq, const KVCache& kv, int64_t n_s
            void* out, int64_t ldo, int64_t B, int64_t nh, int64_t nkv, int64_t hd, float scale, int splits, float* ws,
            unsigned* err, cudaStream_t st);
 }  // namespace decode
+
+// kv_quant.cu. sc: scales of an 8-bit cache, or nullptr for a cache in the activation type.
+int rotary_kv_write(int dtype, const void* qkv, int64_t ld, void* q_out, int64_t ldq, const float* cos_t,
+                    const float* sin_t, int64_t rope_rows, int64_t rd, int interleaved, const int64_t* positions,
+                    const KVCache& kv, const KVScales* sc, int64_t B, int64_t T_new, int64_t nh, int64_t nkv,
+                    int64_t hd, int64_t slot_base, int slot_from_pos, cudaStream_t st);
+int kv_dequant(int dtype, const KVCache& kv, const KVScales& sc, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd,
+               void* k_out, void* v_out, cudaStream_t st);
+
+namespace decode_quant {   // attention_decode_quant.cu
+int64_t splits(int64_t n_slots);
+int64_t workspace_bytes(int64_t B, int64_t nh, int64_t hd, int64_t n_slots);
+int launch(int dtype, const void* q, int64_t ldq, const KVCache& kv, const KVScales& sc, int64_t n_slots,
+           const int64_t* positions, void* out, int64_t ldo, int64_t B, int64_t nh, int64_t nkv, int64_t hd, float scale,
+           float* ws, cudaStream_t st);
+}  // namespace decode_quant
 
 }  // namespace fs

@@ -251,6 +251,11 @@ class Scheduler:
             req.blocks = []
 
 
+def check_kv_dtype(kv_dtype: Optional[torch.dtype], model_dtype: torch.dtype) -> None:
+    if kv_dtype not in (None, model_dtype, torch.float8_e4m3fn):
+        raise ValueError(f"kv_dtype must be the model's dtype ({model_dtype}) or torch.float8_e4m3fn, not {kv_dtype}")
+
+
 class _DecodeGraph:
     """One decode step of `rows` greedy rows (one new token each) captured as a CUDA graph: embedding, every layer,
     final norm, head of the last position and argmax, over static device buffers for the token ids, positions and
@@ -374,6 +379,9 @@ class Engine(Scheduler):
     back, without a host synchronisation per step. A tensor-parallel model (its all-reduces run through
     torch.distributed) always launches eagerly and steps one at a time.
 
+    kv_dtype=torch.float8_e4m3fn (extra): an 8-bit block pool (PagedKVPool), half the cache bytes of bf16, so twice the
+    blocks in the same memory; keys and values are rounded as they are written.
+
     Under tensor parallelism every shard runs the same Engine over its own model shard (model.tp): the pool holds
     the shard's KV heads, the logits are replicated, so every shard samples the same tokens (engine.py:36-45 with
     the TP model of model.py:112)."""
@@ -382,9 +390,11 @@ class Engine(Scheduler):
     MAX_WINDOW = 64     # decode steps per window: bounds what the host enqueues ahead of the GPU
 
     def __init__(self, model, num_blocks: int, block_size: int = 16, max_batch: int = 8, seed: int = 0,
-                 cuda_graphs: bool = True):
+                 cuda_graphs: bool = True, kv_dtype: Optional[torch.dtype] = None):
         self.model, self.cfg = model, model.cfg
-        self.pool = PagedKVPool(self.cfg, num_blocks, block_size, tp=model.tp, dtype=model.dtype, device=model.device)
+        check_kv_dtype(kv_dtype, model.dtype)
+        self.pool = PagedKVPool(self.cfg, num_blocks, block_size, tp=model.tp, dtype=kv_dtype or model.dtype,
+                                device=model.device)
         self.cuda_graphs = cuda_graphs
         self._graphs: Dict[int, _DecodeGraph] = {}
         self.windows = 0    # decode windows run (see _decode_window)

@@ -19,6 +19,7 @@ with the reference's rounding points kept in every kernel (see csrc/). Tensors m
 there is no CPU implementation.
 """
 
+import math
 from typing import List, Optional
 
 import torch
@@ -26,7 +27,7 @@ import torch.nn as nn
 
 from . import _lib as L
 from . import ops
-from .config import ModelConfig
+from .config import ModelConfig, check_rope_scaling
 from .kv import ContiguousKV, new_contiguous_cache, row_table
 from .paged import PagedLayerView
 from .parallel import SINGLE, TPContext
@@ -49,11 +50,46 @@ def precompute_rope(head_dim: int, max_len: int, theta: float):
     return angles.cos(), angles.sin()
 
 
+def rope_frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = None):
+    """(angle per position of each pair in 64 bits, factor on cos and sin) of a scaled rotary form:
+
+    linear     every angle divided by the factor (positions interpolated)
+    ntk        base theta * factor^(r / (r - 2)): the fastest pair keeps its angle, the slowest is divided by the factor
+    by_parts   pairs that turn more than beta_fast times within original_max_len keep their angle, pairs that turn less
+               than beta_slow times are divided by the factor, those between are blended; cos and sin times attn_factor
+    """
+    check_rope_scaling(scaling)
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    kind, factor = (None, 1.0) if scaling is None else (scaling["kind"], float(scaling["factor"]))
+    if kind == "ntk" and rotary_dim > 2:
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = theta ** (-i / rotary_dim)
+    if kind == "linear" or (kind == "ntk" and rotary_dim <= 2):
+        return freq / factor, 1.0
+    if kind == "by_parts":
+        slow, fast = float(scaling.get("beta_slow", 1.0)), float(scaling.get("beta_fast", 32.0))
+        turns = scaling["original_max_len"] * freq / (2 * math.pi)
+        keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
+        return freq * (keep + (1.0 - keep) / factor), float(scaling.get("attn_factor", 1.0))
+    return freq, 1.0
+
+
+def rope_tables(rotary_dim: int, max_len: int, theta: float, scaling: Optional[dict] = None):
+    """cos/sin tables (max_len, rotary_dim/2) in fp32 of rope_frequencies, the angles taken in 64 bits (at position
+    100000 an fp32 angle is off by up to 0.004)."""
+    freq, factor = rope_frequencies(rotary_dim, theta, scaling)
+    angles = torch.arange(max_len, dtype=torch.float64)[:, None] * freq
+    return (angles.cos() * factor).float(), (angles.sin() * factor).float()
+
+
 class RopeTables:
     """fp32 cos/sin tables per device; the kernels round them to the activation dtype as the reference does."""
 
     def __init__(self, cfg: ModelConfig):
-        self.cos, self.sin = precompute_rope(cfg.head_dim, cfg.max_seq_len, cfg.rope_theta)
+        if cfg.rope_scaling is None and cfg.rotary_width == cfg.head_dim:
+            self.cos, self.sin = precompute_rope(cfg.head_dim, cfg.max_seq_len, cfg.rope_theta)
+        else:
+            self.cos, self.sin = rope_tables(cfg.rotary_width, cfg.max_seq_len, cfg.rope_theta, cfg.rope_scaling)
         self._dev = {}
 
     def on(self, device: torch.device):
@@ -101,6 +137,9 @@ class Attention(nn.Module):
         self.hd = cfg.head_dim
         self.nh, self.nkv = cfg.n_heads // tp.size, cfg.n_kv_heads // tp.size
         self.rep = cfg.n_heads // cfg.n_kv_heads
+        self.rope_layout = cfg.rope_layout
+        # the reference's form (half layout, whole head) keeps its own kernel and bf16 rounding points
+        self.plain_rope = cfg.rope_layout == "half" and cfg.rotary_width == cfg.head_dim
         f = dict(bias=False, device=device, dtype=dtype)
         self.wq = nn.Linear(cfg.d_model, self.nh * self.hd, **f)
         self.wk = nn.Linear(cfg.d_model, self.nkv * self.hd, **f)
@@ -137,12 +176,23 @@ def _bind_kv(kv, B: int, T: int, nkv: int, hd: int, dtype, device, positions: to
         table = row_table(B, device)
         return ops.contiguous_desc(k, v, table), base + T, base, False, (lambda: kv.commit(T)), (k, v, table)
     if isinstance(kv, PagedLayerView):
-        if kv.pool.k[kv.layer].dtype != dtype or kv.pool.device != torch.device(device):
+        pool_dtype = torch.float8_e4m3fn if kv.pool.quantized else dtype
+        if kv.pool.k[kv.layer].dtype != pool_dtype or kv.pool.device != torch.device(device):
             raise ValueError("paged pool dtype/device differs from the model's")
         if kv.positions.shape != positions.shape:
             raise ValueError("paged view positions must match the step's positions")
         return kv.descriptor(), kv.n_slots, 0, True, (lambda: None), (kv.tables,)
     return None
+
+
+def _rope_write(a: "Attention", qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, desc,
+                B: int, T: int, slot_base: int, slot_from_pos: bool) -> None:
+    """Rotate q and k of a layer's projections in place and store k and v in the cache."""
+    if a.plain_rope and not isinstance(desc, L.KVQuantDesc):
+        ops.rope_kv_write(qkv, cos, sin, positions, desc, B, T, a.nh, a.nkv, a.hd, slot_base, slot_from_pos)
+    else:
+        ops.rotary_kv_write(qkv, cos, sin, positions, desc, B, T, a.nh, a.nkv, a.hd, slot_base, slot_from_pos,
+                            layout=a.rope_layout)
 
 
 def layer_forward_(blk: "Block", x: torch.Tensor, positions: torch.Tensor, kv, rope_cos: torch.Tensor,
@@ -162,18 +212,25 @@ def layer_forward_(blk: "Block", x: torch.Tensor, positions: torch.Tensor, kv, r
         ks = torch.empty(B, nkv, T, hd, dtype=x.dtype, device=x.device)
         vs = torch.empty_like(ks)
         table = row_table(B, x.device)
-        ops.rope_kv_write(qkv2, rope_cos, rope_sin, positions, ops.contiguous_desc(ks, vs, table), B, T, nh, nkv,
-                          hd, slot_base=0, slot_from_pos=False)
+        _rope_write(a, qkv2, rope_cos, rope_sin, positions, ops.contiguous_desc(ks, vs, table), B, T, slot_base=0,
+                    slot_from_pos=False)
         k_all, v_all = kv.update(ks, vs)
         k_all, v_all = k_all.contiguous(), v_all.contiguous()
         desc, n_slots = ops.contiguous_desc(k_all, v_all, table), k_all.shape[2]
         keep = (k_all, v_all, table)
     else:
         desc, n_slots, base, from_pos, commit, keep = bound
-        ops.rope_kv_write(qkv2, rope_cos, rope_sin, positions, desc, B, T, nh, nkv, hd, slot_base=base,
-                          slot_from_pos=from_pos)
+        _rope_write(a, qkv2, rope_cos, rope_sin, positions, desc, B, T, slot_base=base, slot_from_pos=from_pos)
+    quant = isinstance(desc, L.KVQuantDesc)
+    if quant and T > 1:
+        # several new tokens a row over an 8-bit cache: attention over the visible slots read back as dense tensors
+        k_all, v_all = ops.kv_dequant(desc, B, n_slots, nkv, hd, x.dtype)
+        table = row_table(B, x.device)
+        desc, keep = ops.contiguous_desc(k_all, v_all, table), (keep, k_all, v_all, table)
     attn = torch.empty(B, T, nh * hd, dtype=x.dtype, device=x.device)
-    if T == 1 and hd in (64, 128) and nh // nkv <= 8:
+    if quant and T == 1:
+        ops.attention_decode_quant(qkv2[:, : nh * hd], desc, n_slots, positions, attn.view(M, nh * hd), B, nh, nkv, hd)
+    elif T == 1 and hd in (64, 128) and nh // nkv <= 8:
         # one new token per row (decode): split-KV kernel reading each K/V row once per KV head
         ops.attention_decode(qkv2[:, : nh * hd], desc, n_slots, positions, attn.view(M, nh * hd), B, nh, nkv, hd)
     else:

@@ -242,6 +242,130 @@ def paged_gather(pool: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _row_view(t: torch.Tensor, rows: int, cols: int, name: str) -> int:
+    """Row stride of t seen as `rows` rows of `cols` values; refuses other sizes and rows that overlap."""
+    n, stride = _rows(t)
+    if n != rows or t.shape[-1] != cols:
+        raise ValueError(f"{name} must hold {rows} rows of {cols} values, not {tuple(t.shape)}")
+    if n > 1 and next(t.stride(i) for i in range(t.dim() - 2, -1, -1) if t.shape[i] > 1) < cols:
+        raise ValueError(f"the rows of {name} overlap")
+    return stride
+
+
+def _check_positions(positions: torch.Tensor, n: int) -> None:
+    if positions.dtype != torch.int64 or not positions.is_contiguous() or positions.numel() != n:
+        raise ValueError(f"positions must be {n} contiguous int64 values")
+
+
+def _on_device(device: torch.device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            require_cuda(t)
+            raise RuntimeError(f"tensors on two devices: {device} and {t.device}")
+
+
+def _check_cache(kv, B: int, nkv: int, hd: int, device: torch.device, dtype: torch.dtype) -> None:
+    """The tensors behind a descriptor against a call's sizes (descriptors filled by hand carry none)."""
+    keep = getattr(kv, "keep", None)
+    if keep is None:
+        return
+    k, v, table = keep[:3]
+    _on_device(device, k, v, table)
+    if k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f"the cache holds {k.dtype}, the call needs {dtype}")
+    if k.shape[1] != nkv or k.shape[3] != hd or k.shape != v.shape:
+        raise ValueError(f"the cache holds {k.shape[1]} heads of {k.shape[3]}, the call has {nkv} of {hd}")
+    if table.dtype != torch.int64 or table.numel() and table.stride(-1) != 1:
+        raise ValueError("the block table must be int64 with contiguous rows")
+    if table.shape[0] < B:
+        raise ValueError(f"the block table has {table.shape[0]} rows, the call {B}")
+
+
+_ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+def rotary_kv_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                    positions: torch.Tensor, kv, B: int, T: int, nh: int, nkv: int, hd: int, slot_base: int = 0,
+                    slot_from_pos: bool = True, layout: str = "half",
+                    q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotate q and k of the fused q/k/v rows (B*T, (nh + 2 nkv) * hd) and store k and v into the cache.
+
+    cos, sin: fp32 (positions, r/2); the first r values of each head turn, in pairs (x[i], x[i + r/2]) (layout "half")
+    or (x[2i], x[2i+1]) ("interleaved"); None rotates nothing. fp32 arithmetic with one rounding, where rope_kv_write
+    keeps the reference's bf16 roundings. kv: paged_desc / contiguous_desc (a cache in qkv's dtype) or
+    quant_paged_desc (an 8-bit cache). Returns the rotated q: q_out (B*T, nh * hd), or q's place in qkv, rotated in
+    place. A negative position marks padding: its q_out row and the cache stay as they were. Two tokens of a call must
+    not share a slot."""
+    require_cuda(qkv)
+    dev, M = qkv.device, B * T
+    ld = _row_view(qkv, M, (nh + 2 * nkv) * hd, "qkv")
+    code = dtype_code(qkv.dtype)
+    if layout not in _ROPE_LAYOUTS:
+        raise ValueError(f"layout must be 'half' or 'interleaved', not {layout!r}")
+    _check_positions(positions, M)
+    _on_device(dev, positions, cos, sin, q_out)
+    rows = rd = 0
+    if cos is not None or sin is not None:
+        if (cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32
+                or sin.dtype != torch.float32 or not cos.is_contiguous() or not sin.is_contiguous()):
+            raise ValueError("cos and sin must be contiguous fp32 tables of one shape (positions, rotary_dim / 2)")
+        rows, rd = cos.shape[0], 2 * cos.shape[1]
+    if q_out is None:
+        q_out = qkv.reshape(M, -1)[:, : nh * hd] if qkv.dim() != 2 else qkv[:, : nh * hd]
+        ldq = ld
+    else:
+        if q_out.dtype != qkv.dtype:
+            raise TypeError("q_out must have qkv's dtype")
+        ldq = _row_view(q_out, M, nh * hd, "q_out") if nh else 0
+    quant = isinstance(kv, L.KVQuantDesc)
+    _check_cache(kv, B, nkv, hd, dev, torch.float8_e4m3fn if quant else qkv.dtype)
+    lib = L.load()
+    with torch.cuda.device(dev):
+        L.check((lib.fs_rotary_kv_write_quant if quant else lib.fs_rotary_kv_write)(
+            _p(qkv), ld, _p(q_out), ldq, _p(cos), _p(sin), rows, rd, _ROPE_LAYOUTS[layout], _p(positions),
+            ctypes.byref(kv), B, T, nh, nkv, hd, slot_base, int(slot_from_pos), code, _stream(qkv)),
+            "fs_rotary_kv_write")
+    return q_out
+
+
+def kv_dequant(kv: L.KVQuantDesc, B: int, n_slots: int, nkv: int, hd: int, dtype: torch.dtype):
+    """The first n_slots slots of every row of an 8-bit cache as dense (k, v), each (B, nkv, n_slots, hd) of dtype."""
+    dev = kv.keep[0].device
+    require_cuda(kv.keep[0])
+    code = dtype_code(dtype)
+    _check_cache(kv, B, nkv, hd, dev, torch.float8_e4m3fn)
+    k = torch.empty(B, nkv, n_slots, hd, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    with torch.cuda.device(dev):
+        L.check(L.load().fs_kv_dequant(ctypes.byref(kv), B, n_slots, nkv, hd, _p(k), _p(v), code, _stream(k)),
+                "fs_kv_dequant")
+    return k, v
+
+
+def attention_decode_quant(q: torch.Tensor, kv: L.KVQuantDesc, n_slots: int, positions: torch.Tensor,
+                           out: torch.Tensor, B: int, nh: int, nkv: int, hd: int) -> torch.Tensor:
+    """attention_decode over an 8-bit cache: one query per row (positions (B,) or (B, 1)), any n_heads / n_kv_heads,
+    even head_dim up to 256. A row with a negative position sees no slot and gets zeros."""
+    require_cuda(q)
+    dev = q.device
+    _on_device(dev, positions, out)
+    if out.dtype != q.dtype:
+        raise TypeError("attention_decode_quant: out must have q's dtype")
+    code = dtype_code(q.dtype)
+    ldq, ldo = _row_view(q, B, nh * hd, "q"), _row_view(out, B, nh * hd, "out")
+    _check_positions(positions, B)
+    _check_cache(kv, B, nkv, hd, dev, torch.float8_e4m3fn)
+    lib = L.load()
+    need = lib.fs_attention_decode_quant_workspace(B, nh, hd, n_slots)
+    # Allocated by each call: the allocator hands it out in stream order, and a captured call's stays with its graph.
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    with torch.cuda.device(dev):
+        L.check(lib.fs_attention_decode_quant(_p(q), ldq, ctypes.byref(kv), n_slots, _p(positions), _p(out), ldo, B, nh,
+                                              nkv, hd, 1.0 / math.sqrt(hd), _p(ws), need, code, _stream(q)),
+                "fs_attention_decode_quant")
+    return out
+
+
 def embed(ids: torch.Tensor, table: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """table[ids] for int64 ids on the table's device (nn.Embedding)."""
     require_cuda(ids, table)
@@ -279,4 +403,28 @@ def paged_desc(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> L.KVCac
     desc = L.KVCacheDesc(k.data_ptr(), v.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], bs,
                          nkv * bs * hd, bs * hd, nblk)
     desc.keep = (k, v, table)
+    return desc
+
+
+def quant_paged_desc(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                     table: torch.Tensor) -> L.KVQuantDesc:
+    """Descriptor of an 8-bit paged pool: codes k, v float8_e4m3fn (num_blocks, nkv, block_size, hd), scales fp32
+    (num_blocks, nkv, block_size); table (B, nb) int64."""
+    nblk, nkv, bs, hd = k.shape
+    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+        raise TypeError("quant_paged_desc: k and v must be float8_e4m3fn")
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise TypeError("quant_paged_desc: the scales must be float32")
+    if v.shape != k.shape or k_scale.shape != k.shape[:3] or v_scale.shape != k.shape[:3]:
+        raise ValueError("quant_paged_desc: k, v and their scales must describe one pool")
+    s0, s1, s2, s3 = k.stride()
+    c0, c1, c2 = k_scale.stride()
+    if v.stride() != k.stride() or v_scale.stride() != k_scale.stride() or (s2, s3, c2) != (hd, 1, 1):
+        raise ValueError("quant_paged_desc: the slots of a (block, head) must lie contiguously, k and v alike")
+    if table.dim() != 2:
+        raise ValueError("quant_paged_desc: the block table must be 2-D")
+    _on_device(k.device, v, k_scale, v_scale, table)
+    desc = L.KVQuantDesc(L.KVCacheDesc(k.data_ptr(), v.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], bs,
+                                       s0, s1, nblk), k_scale.data_ptr(), v_scale.data_ptr(), c0, c1)
+    desc.keep = (k, v, table, k_scale, v_scale)
     return desc

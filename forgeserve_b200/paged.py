@@ -44,7 +44,10 @@ class BlockAllocator:
 class PagedKVPool:
     """The block pool of every layer; shapes (num_blocks, kv_heads_of_this_shard, block_size, head_dim).
 
-    `n_layers` (default cfg.n_layers) lets a pipeline stage hold a pool for its own layers only."""
+    `n_layers` (default cfg.n_layers) lets a pipeline stage hold a pool for its own layers only.
+
+    dtype=torch.float8_e4m3fn (extra): an 8-bit pool. `k` and `v` hold e4m3 codes and `k_scale` / `v_scale` one fp32
+    scale for each (block, KV head, slot); a value is code * scale. Layers of any dtype write and read it."""
 
     def __init__(self, cfg: ModelConfig, num_blocks: int, block_size: int = 16, tp: TPContext = SINGLE,
                  dtype=torch.float32, device="cpu", n_layers: Optional[int] = None):
@@ -52,6 +55,10 @@ class PagedKVPool:
         layers = cfg.n_layers if n_layers is None else n_layers
         self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
         self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
+        self.quantized = dtype == torch.float8_e4m3fn
+        if self.quantized:
+            self.k_scale = [torch.zeros(shape[:3], device=device) for _ in range(layers)]
+            self.v_scale = [torch.zeros(shape[:3], device=device) for _ in range(layers)]
         self.block_size = block_size
         self.allocator = BlockAllocator(num_blocks)
 
@@ -85,11 +92,20 @@ class PagedLayerView:
         return self.tables.shape[1] * self.pool.block_size
 
     def descriptor(self):
+        if self.pool.quantized:
+            return ops.quant_paged_desc(self.pool.k[self.layer], self.pool.v[self.layer],
+                                        self.pool.k_scale[self.layer], self.pool.v_scale[self.layer], self.tables)
         return ops.paged_desc(self.pool.k[self.layer], self.pool.v[self.layer], self.tables)
 
     def update(self, k: torch.Tensor, v: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """Store k, v (B, n_kv, T, head_dim) at their positions; return each row's blocks in table order as
         (B, n_kv, max_blocks * block_size, head_dim)."""
+        if self.pool.quantized:
+            B, nkv, T, hd = k.shape
+            rows = torch.stack([k, v]).permute(1, 3, 0, 2, 4).reshape(B * T, 2 * nkv * hd)   # k and v of each token
+            desc = self.descriptor()
+            ops.rotary_kv_write(rows, None, None, self.positions, desc, B, T, 0, nkv, hd)
+            return ops.kv_dequant(desc, B, self.n_slots, nkv, hd, k.dtype)
         ops.kv_store(k, v, self.positions, self.descriptor())
         return ops.paged_gather(self.pool.k[self.layer], self.tables), ops.paged_gather(self.pool.v[self.layer],
                                                                                          self.tables)

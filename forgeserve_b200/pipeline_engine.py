@@ -24,7 +24,7 @@ import torch
 import torch.distributed as dist
 
 from . import ops
-from .engine import Request, Scheduler
+from .engine import Request, Scheduler, check_kv_dtype
 from .paged import PagedKVPool
 from .pipeline import microbatch_sizes, ring_program, seq_pieces
 from .transport import DistTransport, ring_group
@@ -93,16 +93,19 @@ class PipelineEngine(Scheduler):
 
     cuda_graphs (extra, CUDA stages without tensor parallelism): inside decode windows each row group's step on a
     stage replays a captured CUDA graph (_StageDecodeGraph, one per group size) instead of launching every kernel
-    from Python; the same kernels, so the same tokens."""
+    from Python; the same kernels, so the same tokens.
+
+    kv_dtype=torch.float8_e4m3fn (extra): an 8-bit block pool on every stage, as Engine's."""
 
     MAX_WINDOW = 64     # decode steps per window: bounds what the host enqueues ahead of the GPUs
     MAX_GRAPHS = 4
 
     def __init__(self, stage, num_blocks: int, block_size: int = 16, max_batch: int = 8, seed: int = 0,
                  microbatches: int = 1, overlap: Optional[bool] = None, prefill_chunks: int = 1,
-                 cuda_graphs: bool = True):
+                 cuda_graphs: bool = True, kv_dtype: Optional[torch.dtype] = None):
         self.stage, self.cfg = stage, stage.cfg
-        self.pool = PagedKVPool(self.cfg, num_blocks, block_size, tp=stage.tp, dtype=stage.dtype,
+        check_kv_dtype(kv_dtype, stage.dtype)
+        self.pool = PagedKVPool(self.cfg, num_blocks, block_size, tp=stage.tp, dtype=kv_dtype or stage.dtype,
                                 device=stage.device, n_layers=len(stage.layers))
         self.microbatches = max(1, microbatches)
         self.overlap = overlap

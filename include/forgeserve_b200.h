@@ -171,6 +171,53 @@ int fs_attention_decode_static(const void* q, int64_t ldq, const fs_kv_cache* kv
                                const int64_t* positions, void* out, int64_t ldo, int64_t B, int64_t nh, int64_t nkv,
                                int64_t hd, float scale, int dtype, void* stream);
 
+/* ---- Rotary positions in their general form, and the 8-bit KV cache (no counterpart in the reference) ----
+ *
+ * fs_kv_quant: a cache of e4m3 codes. `cache` addresses the codes as fs_kv_cache addresses values (k and v point to
+ * bytes); slot s of row r, KV head g has its scales at table[...] * scale_block_stride + g * scale_head_stride +
+ * s % block_size of k_scale and v_scale. A value is code * scale. */
+typedef struct {
+  fs_kv_cache cache;
+  float* k_scale;
+  float* v_scale;
+  int64_t scale_block_stride;
+  int64_t scale_head_stride;
+} fs_kv_quant;
+
+/* Rotates q and k of the fused q/k/v rows (layout as fs_rope_kv_write) and stores k and v into the cache. The first
+ * rotary_dim values of a head turn (even, 0 .. hd; 0 turns nothing and needs no tables), by tables cos/sin of fp32
+ * (rope_rows, rotary_dim / 2): pairs (x[i], x[i + rotary_dim / 2]), or (x[2i], x[2i+1]) if interleaved != 0. fp32
+ * arithmetic, one rounding (fs_rope_kv_write keeps the reference's bf16 roundings instead). Rotated q goes to rows of
+ * q_out at stride ldq: q's own place (q_out == qkv, ldq == ld), or memory apart from qkv. head_dim even, <= 512. nh may
+ * be 0. A negative position marks a padding token: its q_out row and the cache are left as they are. Two tokens of one
+ * call must not share a slot: which of them a shared slot then holds, or in what mixture, is not defined.
+ *   fs_rotary_kv_write: the cache holds values of `dtype`.
+ *   fs_rotary_kv_write_quant: the cache holds codes. Each (token, KV head) row of k and of v gets the scale
+ *     max(max|x| / 448, 2^-126) and the codes e4m3(x / scale), nearest even; a row with an infinity or a NaN reads back
+ *     as NaN. */
+int fs_rotary_kv_write(const void* qkv, int64_t ld, void* q_out, int64_t ldq, const float* cos_t, const float* sin_t,
+                       int64_t rope_rows, int64_t rotary_dim, int interleaved, const int64_t* positions,
+                       const fs_kv_cache* kv, int64_t B, int64_t T, int64_t nh, int64_t nkv, int64_t hd,
+                       int64_t slot_base, int slot_from_pos, int dtype, void* stream);
+int fs_rotary_kv_write_quant(const void* qkv, int64_t ld, void* q_out, int64_t ldq, const float* cos_t,
+                             const float* sin_t, int64_t rope_rows, int64_t rotary_dim, int interleaved,
+                             const int64_t* positions, const fs_kv_quant* kv, int64_t B, int64_t T, int64_t nh,
+                             int64_t nkv, int64_t hd, int64_t slot_base, int slot_from_pos, int dtype, void* stream);
+
+/* k_out, v_out (B, nkv, n_slots, hd) of `dtype` = code * scale of slots 0 .. n_slots-1 of every row; a block number
+ * outside the cache reads as zeros and flags FS_ERR_BAD_SLOT. */
+int fs_kv_dequant(const fs_kv_quant* kv, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd, void* k_out, void* v_out,
+                  int dtype, void* stream);
+
+/* fs_attention_decode over an 8-bit cache: one query a row, any n_heads / n_kv_heads, head_dim even and <= 256. A row
+ * with a negative position sees no slot and gets zeros. workspace: fs_attention_decode_quant_workspace(...) bytes (0 up
+ * to 512 slots), 16-byte aligned, as for fs_attention_decode. */
+int64_t fs_attention_decode_quant_workspace(int64_t B, int64_t nh, int64_t hd, int64_t n_slots);
+int fs_attention_decode_quant(const void* q, int64_t ldq, const fs_kv_quant* kv, int64_t n_slots,
+                              const int64_t* positions, void* out, int64_t ldo, int64_t B, int64_t nh, int64_t nkv,
+                              int64_t hd, float scale, void* workspace, int64_t workspace_bytes, int dtype,
+                              void* stream);
+
 /* Token embedding gather out[i] = table[ids[i]] (nn.Embedding at pipeline.py:106 / model.py:134-135). */
 int fs_embed(const int64_t* ids, int64_t n, const void* table, int64_t vocab, int64_t dim, void* out, int dtype,
              void* stream);
