@@ -207,6 +207,13 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// 2^x, 2^-22 of the value off at most; results below 2^-126 are zero.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // vs as mantissa * 2^e; zero gives e = -infinity, infinity and NaN themselves. Scales are not negative.
 __device__ __forceinline__ void split_scale(float vs, float& e, float& mant) {
   const uint32_t b = __float_as_uint(vs);
@@ -219,33 +226,36 @@ __device__ __forceinline__ void split_scale(float vs, float& e, float& mant) {
   }
 }
 
-template <typename T, int HD, int NT>
+// WHOLE: the block size is a multiple of 16, so a tile lies in one block and its rows follow one another; otherwise
+// every key is looked up by itself.
+template <typename T, int HD, int NT, bool WHOLE>
 struct Geo {
   static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;        // f16 terms of q and of p
   static constexpr int KS = HD / 16;                          // k steps of S^T, and m tiles of O^T
   static constexpr int KC = HD / 64;                          // 16-byte chunks a lane takes of a K row
   static constexpr int VB = HD / 8 < 16 ? 8 : 16;             // bytes of one V copy
   static constexpr int VC = HD / 8 / VB;                      // V copies a key
-  static constexpr int STAGES = 3;
+  static constexpr int STAGES = 2;
+  static constexpr bool Q_REGS = NT * PARTS * KS <= 8;        // q's operands in registers, else read from shared memory
   static constexpr int V_OFF = 2 * KC * 512;                  // slot: K copies, V copies (32 lanes each), 32 scales
   static constexpr int S_OFF = V_OFF + 4 * VC * VB * 32;
   static constexpr int SLOT = S_OFF + 128;
   static constexpr int RING = WARPS * STAGES * SLOT;
   static constexpr int Q_OFF = RING;                          // q as B operands: [NT][PARTS][KS][32 lanes] of 8 bytes
   static constexpr int Q_BYTES = NT * PARTS * KS * 256;
-  static constexpr int AT_OFF = Q_OFF + Q_BYTES;              // offsets of a warp's keys: values, then scales
-  static constexpr int AT_BYTES = WARPS * TILES * TILE * 16;
-  static constexpr int H_OFF = AT_OFF + AT_BYTES;             // [8 NT] score factors
-  static constexpr int SMEM = H_OFF + 8 * NT * 4;
-  static constexpr int O_BYTES = WARPS * 8 * NT * (HD + 2) * 4;   // the warps' sums, then (max, sum): over ring, q, offsets
-  static_assert(O_BYTES <= H_OFF, "the merge area must fit");
+  static constexpr int AT_OFF = Q_OFF + Q_BYTES;              // offsets of a warp's tiles or keys: values, then scales
+  static constexpr int AT_N = WARPS * TILES * (WHOLE ? 1 : TILE);
+  static constexpr int H_OFF = AT_OFF + AT_N * 16;            // [8 NT] score factors
+  static constexpr int O_ROW = HD + 4;                        // padded: the lanes' writes spread over the banks
+  static constexpr int O_BYTES = WARPS * 8 * NT * (O_ROW + 2) * 4;   // the warps' sums, then (max, sum), over all that
+  static constexpr int SMEM = O_BYTES > H_OFF + 32 * NT ? O_BYTES : H_OFF + 32 * NT;
 };
 
-template <typename T, int HD, int NT>
+template <typename T, int HD, int NT, bool WHOLE>
 __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
   pdl_trigger();
   pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
-  using G = Geo<T, HD, NT>;
+  using G = Geo<T, HD, NT, WHOLE>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, tl = lane & 3;
   const int split = blockIdx.x, kvh = blockIdx.y / p.groups, h0 = (blockIdx.y % p.groups) * 8 * NT;
@@ -263,14 +273,15 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
   const int n_tiles = (n_keys + TILE - 1) / TILE;
   const int my_n = n_tiles > warp ? (n_tiles - warp + WARPS - 1) / WARPS : 0;   // tiles warp, warp + 4, ..
 
-  // Where this warp's keys lie, -1 for a key that is not visible or whose block is bad.
-  int64_t* at = reinterpret_cast<int64_t*>(smem + G::AT_OFF) + warp * TILES * TILE;
-  int64_t* sat = at + WARPS * TILES * TILE;
+  // Where this warp's tiles (or keys) begin, -1 for a key that is not visible or whose block is bad.
+  constexpr int PER = WHOLE ? 1 : TILE, LOOK = TILES * PER;
+  int64_t* at = reinterpret_cast<int64_t*>(smem + G::AT_OFF) + warp * LOOK;
+  int64_t* sat = at + WARPS * LOOK;
 #pragma unroll
-  for (int i = 0; i < TILES * TILE / 32; ++i) {
-    const int k = lane + 32 * i, key = (warp + WARPS * (k / TILE)) * TILE + k % TILE;
+  for (int i = 0; i < (LOOK + 31) / 32; ++i) {
+    const int k = lane + 32 * i, key = (warp + WARPS * (k / PER)) * TILE + k % PER;
     int64_t a = -1, b = -1;
-    if (key < n_keys) {
+    if (key < n_keys && k < LOOK) {
       int64_t col, in;
       split_slot(begin + key, p.kv.block_size, col, in);
       const int64_t blk = col < p.kv.table_cols ? p.kv.table[r * p.kv.table_stride + col] : -1;
@@ -281,8 +292,10 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
         flag_error(p.err, ERR_BAD_SLOT);
       }
     }
-    at[k] = a;
-    sat[k] = b;
+    if (k < LOOK) {
+      at[k] = a;
+      sat[k] = b;
+    }
   }
   __syncwarp();
 
@@ -291,26 +304,51 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
   const float* sbase = lane < TILE ? p.sc.k : p.sc.v;
   uint8_t* ring = smem + warp * G::STAGES * G::SLOT;
   auto issue = [&](int j) {   // tile j of this warp into slot j % STAGES
-    uint8_t* slot = ring + (j % G::STAGES) * G::SLOT;
-    const uint32_t dst = smem_u32(slot) + lane * 16;
-    const int64_t* a = at + j * TILE;
+    const uint32_t slot = smem_u32(ring) + (j % G::STAGES) * G::SLOT;
+    const uint32_t dst = slot + lane * 16, vdst = slot + G::V_OFF + lane * G::VB;
+    if constexpr (WHOLE) {
+      const int64_t o = at[j], so = sat[j];
+      const int n = o < 0 ? 0 : n_keys - (warp + WARPS * j) * TILE;   // rows to read; the rest become zeros
+      const uint8_t* kp = kbase + (o < 0 ? 0 : o) + tl * 16;
+      const uint8_t* vp = vbase + (o < 0 ? 0 : o) + gl * (HD / 8);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int64_t o = a[gl + 8 * i];
+      for (int i = 0; i < 2; ++i) {
+        const bool ok = gl + 8 * i < n;
+        const uint8_t* src = ok ? kp + (gl + 8 * i) * HD : kbase;
 #pragma unroll
-      for (int c = 0; c < G::KC; ++c)
-        copy_async<16>(dst + (i * G::KC + c) * 512, kbase + (o < 0 ? 0 : o + (tl + 4 * c) * 16), o >= 0);
+        for (int c = 0; c < G::KC; ++c) copy_async<16>(dst + (i * G::KC + c) * 512, src + c * 64, ok);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 2 * tl + (i & 1) + 8 * (i >> 1);
+        const bool ok = key < n;
+        const uint8_t* src = ok ? vp + key * HD : vbase;
+#pragma unroll
+        for (int c = 0; c < G::VC; ++c)
+          copy_async<G::VB>(vdst + (i * G::VC + c) * 32 * G::VB, src + c * G::VB, ok);
+      }
+      const bool ok = (lane & (TILE - 1)) < n;
+      copy_async<4>(slot + G::S_OFF + lane * 4, sbase + (ok ? so + (lane & (TILE - 1)) : 0), ok);
+    } else {
+      const int64_t* a = at + j * TILE;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t o = a[gl + 8 * i];
+#pragma unroll
+        for (int c = 0; c < G::KC; ++c)
+          copy_async<16>(dst + (i * G::KC + c) * 512, kbase + (o < 0 ? 0 : o + (tl + 4 * c) * 16), o >= 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t o = a[2 * tl + (i & 1) + 8 * (i >> 1)];
+#pragma unroll
+        for (int c = 0; c < G::VC; ++c)
+          copy_async<G::VB>(vdst + (i * G::VC + c) * 32 * G::VB, vbase + (o < 0 ? 0 : o + gl * (HD / 8) + c * G::VB),
+                            o >= 0);
+      }
+      const int64_t so = sat[j * TILE + (lane & (TILE - 1))];
+      copy_async<4>(slot + G::S_OFF + lane * 4, sbase + (so < 0 ? 0 : so), so >= 0);
     }
-    const uint32_t vdst = smem_u32(slot) + G::V_OFF + lane * G::VB;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t o = a[2 * tl + (i & 1) + 8 * (i >> 1)];
-#pragma unroll
-      for (int c = 0; c < G::VC; ++c)
-        copy_async<G::VB>(vdst + (i * G::VC + c) * 32 * G::VB, vbase + (o < 0 ? 0 : o + gl * (HD / 8) + c * G::VB), o >= 0);
-    }
-    const int64_t so = sat[j * TILE + (lane & (TILE - 1))];
-    copy_async<4>(smem_u32(slot) + G::S_OFF + lane * 4, sbase + (so < 0 ? 0 : so), so >= 0);
   };
 #pragma unroll
   for (int j = 0; j < G::STAGES; ++j) {
@@ -321,19 +359,20 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
   // Q: warp w scales heads w, w + 4, .. to [1, 2) and lays them out as the lanes' B operands.
   float* hs = reinterpret_cast<float*>(smem + G::H_OFF);
   for (int h = warp; h < 8 * NT; h += WARPS) {
-    float x[HD / 32], top = 0.f;
+    float x[HD / 32];
+    uint32_t top = 0;
     const bool real = h < heads;
     const T* q = static_cast<const T*>(p.q) + r * p.ldq + static_cast<int64_t>(kvh * p.rep + h0 + h) * HD;
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
       x[i] = real ? to_f(q[lane + 32 * i]) : 0.f;
-      top = fmaxf(top, fabsf(x[i]));
+      top = max(top, abs_bits(x[i]));
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // 2^-e of the largest value, in two factors where one would leave fp32's range; no scale for 0 and infinity
-    const int e = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
-    const float f0 = exp2f(static_cast<float>(-(e / 2))), f1 = exp2f(static_cast<float>(-(e - e / 2)));
+    // 2^-e of the largest value as two factors, each inside fp32's range
+    top = __reduce_max_sync(0xffffffffu, top);
+    const int e = top < 0x00800000u ? (top ? -126 : 0) : static_cast<int>(top >> 23) - 127;
+    const int e0 = e >> 1, e1 = e - e0;
+    const float f0 = __int_as_float((127 - e0) << 23), f1 = __int_as_float((127 - e1) << 23);
     __half* dst = reinterpret_cast<__half*>(smem + G::Q_OFF) + static_cast<int64_t>(h >> 3) * G::PARTS * G::KS * 128;
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
@@ -344,20 +383,25 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
       dst[idx] = hi;
       if constexpr (G::PARTS == 2) dst[G::KS * 128 + idx] = __float2half_rn((y - __half2float(hi)) * 2048.f);
     }
-    if (lane == 0) hs[h] = p.scale_log2 / f0 / f1;
+    if (lane == 0) hs[h] = p.scale_log2 * __int_as_float((127 + e0) << 23) * __int_as_float((127 + e1) << 23);
   }
   __syncthreads();
   const uint2* qf = reinterpret_cast<const uint2*>(smem + G::Q_OFF) + lane;
+  uint2 qr[G::Q_REGS ? NT * G::PARTS * G::KS : 1];
+  if constexpr (G::Q_REGS)
+#pragma unroll
+    for (int i = 0; i < NT * G::PARTS * G::KS; ++i) qr[i] = qf[i * 32];
 
   // This lane's columns are heads 8 n + 2 tl and + 1 of each N tile n.
-  float fs[NT][2], m[NT][2], mo[NT][2], l[NT][2], acc[NT][G::KS][4];
+  // ms and mos are the maxima as exponents are taken against them (safe_max).
+  float fs[NT][2], m[NT][2], mo[NT][2], ms[NT][2], mos[NT][2], l[NT][2], acc[NT][G::KS][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       fs[n][c] = hs[8 * n + 2 * tl + c];
       m[n][c] = mo[n][c] = -INFINITY;
-      l[n][c] = 0.f;
+      ms[n][c] = mos[n][c] = l[n][c] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < G::KS; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
@@ -371,11 +415,14 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
     const int k0 = (warp + WARPS * j) * TILE;
     float s[NT][4];
     {
-      float a[NT][G::PARTS][4];
+      // two chains of products, so that one's latency covers the other's
+      float a[NT][G::PARTS][2][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int q = 0; q < G::PARTS; ++q) a[n][q][0] = a[n][q][1] = a[n][q][2] = a[n][q][3] = 0.f;
+        for (int q = 0; q < G::PARTS; ++q)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) a[n][q][c >> 2][c & 3] = 0.f;
 #pragma unroll
       for (int c = 0; c < G::KC; ++c) {
         const uint4 u = *reinterpret_cast<const uint4*>(slot + c * 512 + lane * 16);
@@ -388,8 +435,9 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int q = 0; q < G::PARTS; ++q) {
-              const uint2 b = qf[((n * G::PARTS + q) * G::KS + c * 4 + i) * 32];
-              mma_f16(a[n][q], a0, a1, a2, a3, b.x, b.y);
+              const int at_q = (n * G::PARTS + q) * G::KS + c * 4 + i;
+              const uint2 b = G::Q_REGS ? qr[G::Q_REGS ? at_q : 0] : qf[at_q * 32];
+              mma_f16(a[n][q][i & 1], a0, a1, a2, a3, b.x, b.y);
             }
         }
       }
@@ -397,8 +445,8 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          s[n][c] = a[n][0][c];
-          if constexpr (G::PARTS == 2) s[n][c] = fmaf(a[n][1][c], 1.f / 2048.f, s[n][c]);
+          s[n][c] = a[n][0][0][c] + a[n][0][1][c];
+          if constexpr (G::PARTS == 2) s[n][c] = fmaf(a[n][1][0][c] + a[n][1][1][c], 1.f / 2048.f, s[n][c]);
         }
     }
     // Scores of keys gl (c 0, 1) and gl + 8 (c 2, 3), log2 domain; u: with the exponent of the value's scale.
@@ -428,7 +476,9 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
           }
           t = fmaxf(t, m[n][c]);
           u = fmaxf(u, mo[n][c]);
-          const float cl = exp2f(m[n][c] - safe_max(t)), co = exp2f(mo[n][c] - safe_max(u));
+          ms[n][c] = safe_max(t);
+          mos[n][c] = safe_max(u);
+          const float cl = ex2(m[n][c] - ms[n][c]), co = ex2(mo[n][c] - mos[n][c]);
           l[n][c] *= cl;
 #pragma unroll
           for (int i = 0; i < G::KS; ++i) {
@@ -446,8 +496,8 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const bool in = c < 2 ? in0 : in1;
-        l[n][c & 1] += in ? exp2f(s[n][c] - safe_max(m[n][c & 1])) : 0.f;
-        w[c] = in ? exp2f(s[n][c] + e[c >> 1] - safe_max(mo[n][c & 1])) * mant[c >> 1] : 0.f;
+        l[n][c & 1] += in ? ex2(s[n][c] - ms[n][c & 1]) : 0.f;
+        w[c] = in ? ex2(s[n][c] + e[c >> 1] - mos[n][c & 1]) * mant[c >> 1] : 0.f;
       }
       const uint32_t p0 = pack_half2(w[0], w[1]), p1 = pack_half2(w[2], w[3]);
       pb[n][0][0] = movmatrix_trans(p0);
@@ -503,19 +553,18 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], o);
   __syncthreads();   // ring, q and offsets are free
-  float* osm = reinterpret_cast<float*>(smem);                     // [WARPS][8 NT][HD]
-  float* msm = osm + WARPS * 8 * NT * HD;                          // [WARPS][8 NT][2]
+  float* osm = reinterpret_cast<float*>(smem);                     // [WARPS][8 NT][O_ROW]
+  float* msm = osm + WARPS * 8 * NT * G::O_ROW;                    // [WARPS][8 NT][2]
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int h = warp * 8 * NT + 8 * n + 2 * tl + c;
-      const float f = exp2f(safe_max(mo[n][c]) - safe_max(m[n][c]));
+      const float f = exp2f(mos[n][c] - ms[n][c]);
 #pragma unroll
-      for (int i = 0; i < G::KS; ++i) {
-        osm[h * HD + gl * (HD / 8) + 2 * i] = acc[n][i][c] * f;
-        osm[h * HD + gl * (HD / 8) + 2 * i + 1] = acc[n][i][c + 2] * f;
-      }
+      for (int i = 0; i < G::KS; ++i)
+        *reinterpret_cast<float2*>(osm + h * G::O_ROW + gl * (HD / 8) + 2 * i) =
+            make_float2(acc[n][i][c] * f, acc[n][i][c + 2] * f);
       if (gl == 0) {
         msm[2 * h] = m[n][c];
         msm[2 * h + 1] = l[n][c];
@@ -531,7 +580,7 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
     for (int w = 0; w < WARPS; ++w) {
       const float f = exp2f(msm[2 * (w * 8 * NT + h)] - safe_max(top));
       total += f * msm[2 * (w * 8 * NT + h) + 1];
-      o += f * osm[(w * 8 * NT + h) * HD + d];
+      o += f * osm[(w * 8 * NT + h) * G::O_ROW + d];
     }
     const int hh = kvh * p.rep + h0 + h;
     if (p.splits == 1) {
@@ -554,33 +603,37 @@ bool supported(const Params& p) {
          ((reinterpret_cast<uintptr_t>(p.kv.k) | reinterpret_cast<uintptr_t>(p.kv.v)) & 15) == 0;
 }
 
-template <typename T, int HD, int NT>
-int launch_nt(Params p, int64_t B, int64_t nkv, cudaStream_t st) {
-  using G = Geo<T, HD, NT>;
+template <typename T, int HD, int NT, bool WHOLE>
+int launch_geo(Params p, int64_t B, int64_t nkv, cudaStream_t st) {
+  using G = Geo<T, HD, NT, WHOLE>;
   p.groups = (p.rep + 8 * NT - 1) / (8 * NT);
   if (nkv * p.groups > 65535) return fail("fs_attention_decode_quant: too many heads");
   static bool attr[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr[dev]) {
-    if (cudaFuncSetAttribute(quant_decode_tc_kernel<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) !=
-        cudaSuccess)
+    if (cudaFuncSetAttribute(quant_decode_tc_kernel<T, HD, NT, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             G::SMEM) != cudaSuccess)
       return check_launch("quant_decode_tc set smem");
     attr[dev] = true;
   }
   const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(nkv * p.groups), static_cast<unsigned>(B));
-  launch_pdl_async(quant_decode_tc_kernel<T, HD, NT>, grid, 32 * WARPS, G::SMEM, st, p);
+  launch_pdl_async(quant_decode_tc_kernel<T, HD, NT, WHOLE>, grid, 32 * WARPS, G::SMEM, st, p);
   return check_launch("quant_decode_tc_kernel");
+}
+
+template <typename T, int HD>
+int launch_hd(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
+  const bool whole = p.kv.block_size % TILE == 0;
+  if (p.rep > 8)   // two N tiles read the cache once for up to 16 heads
+    return whole ? launch_geo<T, HD, 2, true>(p, B, nkv, st) : launch_geo<T, HD, 2, false>(p, B, nkv, st);
+  return whole ? launch_geo<T, HD, 1, true>(p, B, nkv, st) : launch_geo<T, HD, 1, false>(p, B, nkv, st);
 }
 
 template <typename T>
 int launch_t(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
-  const bool wide = p.rep > 8;   // two N tiles read the cache once for up to 16 heads
-  switch (p.hd) {
-    case 64: return wide ? launch_nt<T, 64, 2>(p, B, nkv, st) : launch_nt<T, 64, 1>(p, B, nkv, st);
-    case 128: return wide ? launch_nt<T, 128, 2>(p, B, nkv, st) : launch_nt<T, 128, 1>(p, B, nkv, st);
-    default: return wide ? launch_nt<T, 256, 2>(p, B, nkv, st) : launch_nt<T, 256, 1>(p, B, nkv, st);
-  }
+  return p.hd == 64 ? launch_hd<T, 64>(p, B, nkv, st)
+                    : p.hd == 128 ? launch_hd<T, 128>(p, B, nkv, st) : launch_hd<T, 256>(p, B, nkv, st);
 }
 
 }  // namespace tc
