@@ -427,9 +427,9 @@ int fs_kv_dequant(const fs_kv_quant* kv, int64_t B, int64_t n_slots, int64_t nkv
                     static_cast<cudaStream_t>(stream));
 }
 
-int64_t fs_attention_decode_quant_workspace(int64_t B, int64_t nh, int64_t hd, int64_t n_slots) {
-  if (B <= 0 || nh <= 0 || hd <= 0 || n_slots <= 0) return 0;
-  return decode_quant::workspace_bytes(B, nh, hd, n_slots);
+int64_t fs_attention_decode_quant_workspace(int64_t B, int64_t nh, int64_t nkv, int64_t hd, int64_t n_slots) {
+  if (B <= 0 || nh <= 0 || nkv <= 0 || hd <= 0 || n_slots <= 0) return 0;
+  return decode_quant::workspace_bytes(B, nh, nkv, hd, n_slots);
 }
 
 int fs_attention_decode_quant(const void* q, int64_t ldq, const fs_kv_quant* kv, int64_t n_slots,
@@ -449,7 +449,7 @@ int fs_attention_decode_quant(const void* q, int64_t ldq, const fs_kv_quant* kv,
     return fail("fs_attention_decode_quant: n_heads must be a multiple of n_kv_heads");
   if (B > 65535) return fail("fs_attention_decode_quant: too many rows");
   if (ldq < nh * hd || ldo < nh * hd) return fail("fs_attention_decode_quant: row stride too small");
-  const int64_t need = decode_quant::workspace_bytes(B, nh, hd, n_slots);
+  const int64_t need = decode_quant::workspace_bytes(B, nh, nkv, hd, n_slots);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail("fs_attention_decode_quant: workspace of " + std::to_string(need) + " bytes needed");
   if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15))

@@ -6,10 +6,10 @@
 // so a scale is one factor on a score or on a probability, and the products run on the codes themselves.
 // The floor is the cache's bytes: 2 (hd + 4) for each visible slot of each KV head, read once for all its query heads.
 //
-// A row's slots are cut into splits of SPLIT_KEYS, one CTA each, whatever the batch and the table's width, so the order
-// of the sums depends on the row alone (a step gives the same bits eagerly, in a CUDA graph with a padded table, or in
-// micro-batches); quant_combine_kernel joins the splits. Workspace (fp32): sums [B][nh][splits][hd], then (max, sum)
-// [B][nh][splits][2] in the log2 domain.
+// A row's slots are cut into splits, one CTA each; quant_combine_kernel joins them. How they are cut follows from the
+// row's visible slots and the KV heads alone (split_keys), so the order of a row's sums does not depend on the batch or
+// on the table's width (a step gives the same bits eagerly, in a CUDA graph with a padded table, or in micro-batches).
+// Workspace (fp32): sums [B][nh][splits][hd], then (max, sum) [B][nh][splits][2] in the log2 domain.
 //
 // A row with a negative position sees nothing and gets zeros. A block number outside the cache reads as zero rows and
 // flags ERR_BAD_SLOT. Scores of -infinity weigh nothing; a row whose scores all are, or that meets a NaN or +infinity,
@@ -25,8 +25,18 @@ namespace decode_quant {
 
 namespace {
 
-constexpr int SPLIT_KEYS = 512;
-constexpr int HEADS = 8;   // query heads of one KV head that a CTA handles
+constexpr int UNIT_KEYS = 512;   // a split is a multiple of this
+constexpr int ONE_WAVE = 592;    // CTAs that run at once: 4 on each of 148 SMs
+constexpr int HEADS = 8;         // query heads of one KV head that a CTA of the general kernel handles
+
+// Slots a split of a row with n_vis visible slots: 512 while the row's CTAs fit one wave, so that a row alone spreads
+// over the GPU; longer rows get longer splits, which join cheaper (2 rows of 131072 slots of 8 KV heads: 256 splits of
+// 512 took 161 us, 51 of them in the join, 64 of 2048 125 us).
+__host__ __device__ __forceinline__ int64_t split_keys(int64_t n_vis, int64_t nkv) {
+  const int64_t units = (n_vis + UNIT_KEYS - 1) / UNIT_KEYS;
+  const int64_t k = (units * nkv + ONE_WAVE - 1) / ONE_WAVE;
+  return UNIT_KEYS * (k > 1 ? k : 1);
+}
 
 struct Params {
   const void* q;
@@ -37,7 +47,9 @@ struct Params {
   const int64_t* positions;
   void* out;
   int64_t ldo;
-  int nh, rep, hd, splits, groups;   // groups: CTAs a KV head, of HEADS query heads each
+  int nh, nkv, rep, hd, splits, groups;   // groups: CTAs a KV head, of HEADS (or 8 NT) query heads each
+  bool q_vec;                        // rows of q on 16-byte boundaries
+  int rows_per_block, rows_per_head, map_rows;   // of the tensor maps' hd-wide rows (WHOLE)
   float scale_log2;
   float* ws;
   unsigned* err;
@@ -70,8 +82,8 @@ __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
   const int64_t r = blockIdx.z;
   const int heads = p.rep - h0 < HEADS ? p.rep - h0 : HEADS;
   const int64_t n_vis = visible(p, r);
-  const int64_t begin = static_cast<int64_t>(split) * SPLIT_KEYS;
-  const int64_t end = begin + SPLIT_KEYS < n_vis ? begin + SPLIT_KEYS : n_vis;
+  const int64_t per = split_keys(n_vis, p.nkv), begin = split * per;
+  const int64_t end = begin + per < n_vis ? begin + per : n_vis;
   if (begin >= n_vis && !(p.splits == 1 && n_vis == 0)) return;   // the join does not read an empty split
 
   for (int i = tid; i < heads * hd; i += blockDim.x)
@@ -159,24 +171,37 @@ __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
 
 // ------------------------------------------------------------------------------------ tensor-core kernel
 // hd 64, 128 or 256, 16-byte rows. The codes are exact in f16, so both products run as mma.sync m16n8k16 f16 with fp32
-// sums and the scales never touch them:
+// sums and the scales never touch them; the query heads of the KV head are the N side (NT tiles of 8):
 //     S^T (16 keys x 8 heads) = K (16 x hd) Q^T (hd x 8),   O^T (hd x 8 heads) += V^T (hd x 16) P^T (16 x 8)
-// with the query heads of the KV head as the N side (NT tiles of 8). A contraction's index order is free as long as
-// both operands agree, and so are the rows of O^T; they are chosen so that every lane's operand values are 16
-// neighbouring bytes of a cache row: lane (g, t) = (lane / 4, lane % 4) takes, of keys g and g + 8, the 16-byte chunks
-// t, t + 4, .. for K, and of keys 2t, 2t+1, 2t+8, 2t+9 the bytes g hd/8 .. + hd/8 for V. So a lane copies exactly the
-// bytes it will use (cp.async, whole sectors) into slots of its own: a ring in shared memory without barriers, ldmatrix
-// or swizzles, and any block size. P^T reaches the B layout by movmatrix.
+// A contraction's index order is free as long as both operands agree, and so are the rows of O^T; they are chosen so
+// that every lane's operand values are neighbouring bytes of a cache row: lane (g, t) = (lane / 4, lane % 4) takes, of
+// keys g and g + 8, the 16-byte chunks 2t and 2t + 1 of each 128 bytes for K, and of keys 2t, 2t+1, 2t+8, 2t+9 the chunk
+// g for V (8 bytes of it at hd 64). P^T reaches the B layout by movmatrix.
+//
+// A warp takes STEP keys at a time, into a ring of its own; no barrier joins the warps before the end.
+//   WHOLE (the block size is a multiple of 16, so a tile of 16 keys lies in one block): TMA boxes of 16 rows, swizzled over
+//     128 (hd 64: 64) bytes, under which both fragment reads above are free of bank conflicts.
+//   otherwise every key is looked up by itself and each lane copies exactly the bytes it will use (cp.async).
 //
 // Q enters as f16 after a scale by a power of two that brings each head's largest |q| to [1, 2): exact for bf16 down to
 // 2^-14 of it, off by 2^-25 of it below. fp32 queries enter as two halves (a value and its remainder times 2^11): 22
-// bits. P enters as p_j vs_j against a running maximum of its own, so that values whose scales differ widely keep the
-// f16 range: vs = mantissa 2^e, P = exp2(s + e - mo) mantissa, mo >= max(s + e) - SLACK. bf16 rounds P to f16 (2^-11); fp32
-// adds its remainder as a second product. Maxima are raised only when a score exceeds them by SLACK = 2^8: one vote
-// a tile instead of a reduction.
+// bits. P enters in f16 (2^-11) as p_j vs_j against a running maximum of its own, so that values whose scales differ
+// widely keep the f16 range: P = exp2(s + log2 vs - mo), mo >= max(s + log2 vs) - SLACK. fp32 takes log2 vs as exponent
+// and mantissa, and P's remainder as a second product. Maxima are raised only when a score exceeds them by SLACK: one
+// vote a step instead of a reduction.
 namespace tc {
 
-constexpr int WARPS = 4, TILE = 16, TILES = SPLIT_KEYS / TILE / WARPS;   // tiles a warp has of a full split
+#ifndef NWARPS
+#define NWARPS 4
+#endif
+#ifndef NSTAGES
+#define NSTAGES 1
+#endif
+#ifndef MINB
+#define MINB 4
+#endif
+constexpr int WARPS = NWARPS, TILE = 16, STEP = 32;   // a warp takes STEP keys (two tiles) at a time
+constexpr int SEG = UNIT_KEYS / STEP / WARPS;         // steps whose places a warp looks up at once
 constexpr float SLACK = 8.f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -186,12 +211,24 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Orders this thread's earlier shared-memory accesses before later async-proxy (TMA) writes to the same bytes.
+__device__ __forceinline__ void fence_proxy_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// BYTES (4, 8 or 16) from global to shared memory, zeros where !ok.
+// BYTES (4, 8 or 16) from global to shared memory.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+// The same, zeros where !ok (src is then not read, but still a valid address).
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool ok) {
   const int n = ok ? BYTES : 0;
@@ -214,6 +251,41 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// log2(x), off by 2^-22 (of the value where that is more); 0 gives -infinity.
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 neighbouring values as fp32, by 16-byte loads where `vec`.
+__device__ __forceinline__ void load16(const __nv_bfloat16* q, bool vec, float* x) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 u = *reinterpret_cast<const uint4*>(q + 8 * i);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+        x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = to_f(q[i]);
+  }
+}
+__device__ __forceinline__ void load16(const float* q, bool vec, float* x) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(x + 4 * i) = *reinterpret_cast<const float4*>(q + 4 * i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = q[i];
+  }
+}
+
 // vs as mantissa * 2^e; zero gives e = -infinity, infinity and NaN themselves. Scales are not negative.
 __device__ __forceinline__ void split_scale(float vs, float& e, float& mant) {
   const uint32_t b = __float_as_uint(vs);
@@ -226,180 +298,240 @@ __device__ __forceinline__ void split_scale(float vs, float& e, float& mant) {
   }
 }
 
-// WHOLE: the block size is a multiple of 16, so a tile lies in one block and its rows follow one another; otherwise
-// every key is looked up by itself.
 template <typename T, int HD, int NT, bool WHOLE>
 struct Geo {
   static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;        // f16 terms of q and of p
   static constexpr int KS = HD / 16;                          // k steps of S^T, and m tiles of O^T
   static constexpr int KC = HD / 64;                          // 16-byte chunks a lane takes of a K row
-  static constexpr int VB = HD / 8 < 16 ? 8 : 16;             // bytes of one V copy
-  static constexpr int VC = HD / 8 / VB;                      // V copies a key
-  static constexpr int STAGES = 2;
-  static constexpr bool Q_REGS = NT * PARTS * KS <= 8;        // q's operands in registers, else read from shared memory
-  static constexpr int V_OFF = 2 * KC * 512;                  // slot: K copies, V copies (32 lanes each), 32 scales
-  static constexpr int S_OFF = V_OFF + 4 * VC * VB * 32;
-  static constexpr int SLOT = S_OFF + 128;
-  static constexpr int RING = WARPS * STAGES * SLOT;
-  static constexpr int Q_OFF = RING;                          // q as B operands: [NT][PARTS][KS][32 lanes] of 8 bytes
-  static constexpr int Q_BYTES = NT * PARTS * KS * 256;
-  static constexpr int AT_OFF = Q_OFF + Q_BYTES;              // offsets of a warp's tiles or keys: values, then scales
-  static constexpr int AT_N = WARPS * TILES * (WHOLE ? 1 : TILE);
-  static constexpr int H_OFF = AT_OFF + AT_N * 16;            // [8 NT] score factors
+  static constexpr int VB = HD / 8 < 16 ? 8 : 16;             // bytes a lane takes of a V row at once
+  static constexpr int VC = HD / 8 / VB;                      // and how often
+  static constexpr int BOX = HD < 128 ? 64 : 128;             // bytes of a box's row
+  static constexpr int BOXES = HD / BOX;                      // boxes a row
+  static constexpr int STEP_BYTES = STEP * HD;                // K (or V) of a step
+  static constexpr int STAGES = WHOLE ? NSTAGES : 1;
+  static constexpr int BUF = 2 * STAGES * STEP_BYTES;         // a warp's ring: K stages, then V stages
+  static constexpr int Q_OFF = WARPS * BUF;                   // q as B operands: [NT][PARTS][KS][32 lanes] of 8 bytes
+  static constexpr int AT_OFF = Q_OFF + NT * PARTS * KS * 256;   // where tiles or keys lie: [2][values, scales][WARPS][LOOK]
+  static constexpr int LOOK = SEG * (WHOLE ? 2 : STEP);
+  static constexpr int BAR_OFF = AT_OFF + 2 * WARPS * LOOK * 16;   // a warp's barriers: K stages, V stages
+  static constexpr int END = BAR_OFF + (WHOLE ? WARPS * 2 * STAGES * 8 : 0);
   static constexpr int O_ROW = HD + 4;                        // padded: the lanes' writes spread over the banks
-  static constexpr int O_BYTES = WARPS * 8 * NT * (O_ROW + 2) * 4;   // the warps' sums, then (max, sum), over all that
-  static constexpr int SMEM = O_BYTES > H_OFF + 32 * NT ? O_BYTES : H_OFF + 32 * NT;
+  static constexpr int O_BYTES = WARPS * 8 * NT * (O_ROW + 3) * 4;   // the warps' sums, (max, sum), weights, over all that
+  static constexpr int SMEM = (O_BYTES > END ? O_BYTES : END) + (WHOLE ? 1024 : 0);   // boxes lie on 1024 bytes
+  static constexpr int CTAS = NT == 1 && HD <= 128 ? MINB : 1;   // an SM (registers)
+  // byte of a K (or V) step's 16-byte chunk `chunk` of row `row`
+  static __device__ __forceinline__ int box_at(int row, int chunk) {
+    const int tile = row >> 4, r = row & 15;
+    if constexpr (BOX == 64) return tile * 16 * HD + r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4);
+    return tile * 16 * HD + (chunk >> 3) * 16 * 128 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+  }
 };
+// The 16-byte chunk of a K row that lane t of a quad takes c-th.
+template <int HD>
+__device__ __forceinline__ int k_chunk(int t, int c) {
+  return HD == 64 ? t : (c >> 1) * 8 + 2 * t + (c & 1);
+}
 
 template <typename T, int HD, int NT, bool WHOLE>
-__global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
+__global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
+    quant_decode_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Params p) {
   pdl_trigger();
-  pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
   using G = Geo<T, HD, NT, WHOLE>;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = WHOLE ? reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023))
+                        : smem_raw;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, tl = lane & 3;
+  uint8_t* buf = smem + warp * G::BUF;
+  uint64_t* kbar = reinterpret_cast<uint64_t*>(smem + G::BAR_OFF) + warp * 2 * G::STAGES;
+  uint64_t* vbar = kbar + G::STAGES;
+  if constexpr (WHOLE) {
+    if (lane == 0) {
+      for (int i = 0; i < 2 * G::STAGES; ++i) mbar_init(&kbar[i], 1);
+      fence_barrier_init();
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+    }
+    __syncwarp();
+  }
+  pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
   const int split = blockIdx.x, kvh = blockIdx.y / p.groups, h0 = (blockIdx.y % p.groups) * 8 * NT;
   const int64_t r = blockIdx.z;
   const int heads = p.rep - h0 < 8 * NT ? p.rep - h0 : 8 * NT;
-  const int64_t n_vis = visible(p, r);
-  const int64_t begin = static_cast<int64_t>(split) * SPLIT_KEYS;
+  const int64_t n_vis = visible(p, r), per = split_keys(n_vis, p.nkv), begin = split * per;
   if (begin >= n_vis) {
     if (p.splits == 1)   // a row that sees nothing
       for (int i = threadIdx.x; i < heads * HD; i += blockDim.x)
         static_cast<T*>(p.out)[r * p.ldo + static_cast<int64_t>(kvh * p.rep + h0) * HD + i] = from_f<T>(0.f);
     return;              // the join does not read an empty split
   }
-  const int n_keys = static_cast<int>(n_vis - begin < SPLIT_KEYS ? n_vis - begin : SPLIT_KEYS);
-  const int n_tiles = (n_keys + TILE - 1) / TILE;
-  const int my_n = n_tiles > warp ? (n_tiles - warp + WARPS - 1) / WARPS : 0;   // tiles warp, warp + 4, ..
+  const int n_keys = static_cast<int>(n_vis - begin < per ? n_vis - begin : per);
+  const int n_steps = (n_keys + STEP - 1) / STEP;
+  const int my_n = n_steps > warp ? (n_steps - warp + WARPS - 1) / WARPS : 0;   // steps warp, warp + WARPS, ..
 
-  // Where this warp's tiles (or keys) begin, -1 for a key that is not visible or whose block is bad.
-  constexpr int PER = WHOLE ? 1 : TILE, LOOK = TILES * PER;
-  int64_t* at = reinterpret_cast<int64_t*>(smem + G::AT_OFF) + warp * LOOK;
-  int64_t* sat = at + WARPS * LOOK;
+  // Where the tiles (a row of the tensor map) or keys of SEG steps of this warp lie, -1 for bad blocks and past the last
+  // visible key. Two segments, so that the next one is looked up while this one is in use.
+  int64_t* at = reinterpret_cast<int64_t*>(smem + G::AT_OFF) + warp * G::LOOK;
+  auto look_up = [&](int seg) {
+    int64_t* dst = at + (seg & 1) * WARPS * G::LOOK * 2;
 #pragma unroll
-  for (int i = 0; i < (LOOK + 31) / 32; ++i) {
-    const int k = lane + 32 * i, key = (warp + WARPS * (k / PER)) * TILE + k % PER;
-    int64_t a = -1, b = -1;
-    if (key < n_keys && k < LOOK) {
-      int64_t col, in;
-      split_slot(begin + key, p.kv.block_size, col, in);
-      const int64_t blk = col < p.kv.table_cols ? p.kv.table[r * p.kv.table_stride + col] : -1;
-      if (blk >= 0 && blk < p.kv.num_blocks) {
-        a = blk * p.kv.block_stride + kvh * p.kv.head_stride + in * HD;
-        b = blk * p.sc.block_stride + kvh * p.sc.head_stride + in;
-      } else {
-        flag_error(p.err, ERR_BAD_SLOT);
+    for (int i = 0; i < (G::LOOK + 31) / 32; ++i) {
+      const int k = lane + 32 * i;
+      const int key = WHOLE ? (warp + WARPS * (seg * SEG + (k >> 1))) * STEP + (k & 1) * TILE
+                            : (warp + WARPS * (seg * SEG + i)) * STEP + lane;
+      if (k < G::LOOK) {
+        int64_t a = -1, b = -1;
+        if (key < n_keys) {
+          int64_t col, in;
+          split_slot(begin + key, p.kv.block_size, col, in);
+          const int64_t blk = col < p.kv.table_cols ? p.kv.table[r * p.kv.table_stride + col] : -1;
+          if (blk >= 0 && blk < p.kv.num_blocks) {
+            a = WHOLE ? blk * p.rows_per_block + kvh * p.rows_per_head + in
+                      : blk * p.kv.block_stride + kvh * p.kv.head_stride + in * HD;
+            b = blk * p.sc.block_stride + kvh * p.sc.head_stride + in;
+          } else {
+            flag_error(p.err, ERR_BAD_SLOT);
+          }
+        }
+        dst[k] = a;
+        dst[WARPS * G::LOOK + k] = b;
       }
     }
-    if (k < LOOK) {
-      at[k] = a;
-      sat[k] = b;
-    }
-  }
-  __syncwarp();
+    __syncwarp();
+  };
+  auto place = [&](int j) -> const int64_t* {   // of step j in `at`
+    return at + ((j / SEG) & 1) * WARPS * G::LOOK * 2 + (j % SEG) * (G::LOOK / SEG);
+  };
 
-  const uint8_t* kbase = static_cast<const uint8_t*>(p.kv.k);
-  const uint8_t* vbase = static_cast<const uint8_t*>(p.kv.v);
-  const float* sbase = lane < TILE ? p.sc.k : p.sc.v;
-  uint8_t* ring = smem + warp * G::STAGES * G::SLOT;
-  auto issue = [&](int j) {   // tile j of this warp into slot j % STAGES
-    const uint32_t slot = smem_u32(ring) + (j % G::STAGES) * G::SLOT;
-    const uint32_t dst = slot + lane * 16, vdst = slot + G::V_OFF + lane * G::VB;
-    if constexpr (WHOLE) {
-      const int64_t o = at[j], so = sat[j];
-      const int n = o < 0 ? 0 : n_keys - (warp + WARPS * j) * TILE;   // rows to read; the rest become zeros
-      const uint8_t* kp = kbase + (o < 0 ? 0 : o) + tl * 16;
-      const uint8_t* vp = vbase + (o < 0 ? 0 : o) + gl * (HD / 8);
+  const uint8_t* none = static_cast<const uint8_t*>(p.kv.k);   // a valid address for copies of nothing
+  const uint64_t once = l2_policy_evict_first();   // each key is read once: leave L2 to the splits' partial sums
+  // One warp's tiles of a step by TMA: rows past the map's end (bad blocks, tiles past the last key) read as zeros.
+  auto load_boxes = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, const int64_t* a) {
+    if (lane == 0) {
+      const int row0 = a[0] < 0 ? p.map_rows : static_cast<int>(a[0]), row1 = a[1] < 0 ? p.map_rows : static_cast<int>(a[1]);
+      fence_proxy_async_smem();   // the warp's reads of the step that lay there come first
+      mbar_arrive_expect_tx(bar, G::STEP_BYTES);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const bool ok = gl + 8 * i < n;
-        const uint8_t* src = ok ? kp + (gl + 8 * i) * HD : kbase;
-#pragma unroll
-        for (int c = 0; c < G::KC; ++c) copy_async<16>(dst + (i * G::KC + c) * 512, src + c * 64, ok);
+      for (int b = 0; b < G::BOXES; ++b) {
+        tma_load_2d_hint(dst + b * 16 * G::BOX, map, bar, b * G::BOX, row0, once);
+        tma_load_2d_hint(dst + 16 * HD + b * 16 * G::BOX, map, bar, b * G::BOX, row1, once);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 2 * tl + (i & 1) + 8 * (i >> 1);
-        const bool ok = key < n;
-        const uint8_t* src = ok ? vp + key * HD : vbase;
-#pragma unroll
-        for (int c = 0; c < G::VC; ++c)
-          copy_async<G::VB>(vdst + (i * G::VC + c) * 32 * G::VB, src + c * G::VB, ok);
-      }
-      const bool ok = (lane & (TILE - 1)) < n;
-      copy_async<4>(slot + G::S_OFF + lane * 4, sbase + (ok ? so + (lane & (TILE - 1)) : 0), ok);
-    } else {
-      const int64_t* a = at + j * TILE;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int64_t o = a[gl + 8 * i];
-#pragma unroll
-        for (int c = 0; c < G::KC; ++c)
-          copy_async<16>(dst + (i * G::KC + c) * 512, kbase + (o < 0 ? 0 : o + (tl + 4 * c) * 16), o >= 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t o = a[2 * tl + (i & 1) + 8 * (i >> 1)];
-#pragma unroll
-        for (int c = 0; c < G::VC; ++c)
-          copy_async<G::VB>(vdst + (i * G::VC + c) * 32 * G::VB, vbase + (o < 0 ? 0 : o + gl * (HD / 8) + c * G::VB),
-                            o >= 0);
-      }
-      const int64_t so = sat[j * TILE + (lane & (TILE - 1))];
-      copy_async<4>(slot + G::S_OFF + lane * 4, sbase + (so < 0 ? 0 : so), so >= 0);
     }
   };
+  // K of this warp's step j; V of it. The warp has read what lay there.
+  auto issue_k = [&](int j) {
+    const int64_t* a = place(j);
+    if constexpr (WHOLE) {
+      load_boxes(&tmK, buf + (j % G::STAGES) * G::STEP_BYTES, &kbar[j % G::STAGES], a);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t o = a[gl + 8 * i];
+        const uint8_t* src = o >= 0 ? static_cast<const uint8_t*>(p.kv.k) + o : none;
+#pragma unroll
+        for (int c = 0; c < G::KC; ++c)
+          copy_async<16>(smem_u32(buf) + ((i * G::KC + c) * 32 + lane) * 16, src + k_chunk<HD>(tl, c) * 16, o >= 0);
+      }
+    }
+  };
+  auto issue_v = [&](int j) {
+    const int64_t* a = place(j);
+    if constexpr (WHOLE) {
+      load_boxes(&tmV, buf + (G::STAGES + j % G::STAGES) * G::STEP_BYTES, &vbar[j % G::STAGES], a);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t o = a[(i >> 2) * TILE + 2 * tl + (i & 1) + 4 * (i & 2)];
+        const uint8_t* src = o >= 0 ? static_cast<const uint8_t*>(p.kv.v) + o : none;
+#pragma unroll
+        for (int c = 0; c < G::VC; ++c)
+          copy_async<G::VB>(smem_u32(buf) + G::STEP_BYTES + ((i * G::VC + c) * 32 + lane) * G::VB,
+                            src + c * 128 + gl * G::VB, o >= 0);
+      }
+    }
+  };
+  float ks_next = 0.f, vs_next = 0.f;   // scales of key `lane` of the next step, zero where it is not visible or bad
+  auto load_scales = [&](int j) {
+    const int64_t* b = place(j) + WARPS * G::LOOK;
+    const int64_t so = WHOLE ? b[lane >> 4] : b[lane];
+    const bool ok = so >= 0 && (warp + WARPS * j) * STEP + lane < n_keys;
+    const int64_t s = so + (WHOLE ? lane & 15 : 0);
+    ks_next = ok ? p.sc.k[s] : 0.f;
+    vs_next = ok ? p.sc.v[s] : 0.f;
+  };
+  auto commit = [] {
+    if constexpr (!WHOLE) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // Waits for K (V) of step j; false if it did not come within the time limit.
+  auto wait = [&](uint64_t* bars, int j) -> bool {
+    if constexpr (WHOLE) {
+      return __all_sync(0xffffffffu, mbar_wait(&bars[j % G::STAGES], static_cast<uint32_t>((j / G::STAGES) & 1), p.err));
+    } else {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      return true;
+    }
+  };
+  look_up(0);
+  if (my_n > 0) load_scales(0);
 #pragma unroll
   for (int j = 0; j < G::STAGES; ++j) {
-    if (j < my_n) issue(j);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (j < my_n) issue_k(j);
+    commit();
+    if (j < my_n) issue_v(j);
+    commit();
   }
 
-  // Q: warp w scales heads w, w + 4, .. to [1, 2) and lays them out as the lanes' B operands.
-  float* hs = reinterpret_cast<float*>(smem + G::H_OFF);
-  for (int h = warp; h < 8 * NT; h += WARPS) {
-    float x[HD / 32];
-    uint32_t top = 0;
-    const bool real = h < heads;
-    const T* q = static_cast<const T*>(p.q) + r * p.ldq + static_cast<int64_t>(kvh * p.rep + h0 + h) * HD;
+  // Q as B operands: lane (gl, tl) holds of head 8 n + gl the dims 16 k_chunk(tl, c) + 4 i + 0..3, k step 4 c + i, after
+  // the head's scale. Every warp finds the scales, and writes its share of the k steps to shared memory.
+  uint2* qf = reinterpret_cast<uint2*>(smem + G::Q_OFF) + lane;
+  float fs[NT][2];   // score factors of this lane's columns, heads 8 n + 2 tl and + 1
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-      x[i] = real ? to_f(q[lane + 32 * i]) : 0.f;
+  for (int n = 0; n < NT; ++n) {
+    const bool real = 8 * n + gl < heads;
+    const T* q = static_cast<const T*>(p.q) + r * p.ldq +
+                 static_cast<int64_t>(kvh * p.rep + h0 + (real ? 8 * n + gl : 0)) * HD;
+    float x[G::KC * 16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < G::KC; ++c) load16(q + k_chunk<HD>(tl, c) * 16, p.q_vec, x + c * 16);
+#pragma unroll
+    for (int i = 0; i < G::KC * 16; ++i) {
+      x[i] = real ? x[i] : 0.f;
       top = max(top, abs_bits(x[i]));
     }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // 2^-e of the largest value as two factors, each inside fp32's range
-    top = __reduce_max_sync(0xffffffffu, top);
-    const int e = top < 0x00800000u ? (top ? -126 : 0) : static_cast<int>(top >> 23) - 127;
-    const int e0 = e >> 1, e1 = e - e0;
+    const int e = top < 0x00800000u ? (top ? -126 : 0) : static_cast<int>(top >> 23) - 127, e0 = e >> 1, e1 = e - e0;
     const float f0 = __int_as_float((127 - e0) << 23), f1 = __int_as_float((127 - e1) << 23);
-    __half* dst = reinterpret_cast<__half*>(smem + G::Q_OFF) + static_cast<int64_t>(h >> 3) * G::PARTS * G::KS * 128;
+    const float back = p.scale_log2 * __int_as_float((127 + e0) << 23) * __int_as_float((127 + e1) << 23);
+    fs[n][0] = __shfl_sync(0xffffffffu, back, 8 * tl);        // lane (2 tl, 0)
+    fs[n][1] = __shfl_sync(0xffffffffu, back, 8 * tl + 4);
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-      const int d = lane + 32 * i, c = d >> 4;
-      const int idx = (((c >> 2) * 4 + ((d & 15) >> 2)) * 32 + (h & 7) * 4 + (c & 3)) * 4 + (d & 3);
-      const float y = x[i] * f0 * f1;
-      const __half hi = __float2half_rn(y);
-      dst[idx] = hi;
-      if constexpr (G::PARTS == 2) dst[G::KS * 128 + idx] = __float2half_rn((y - __half2float(hi)) * 2048.f);
+    for (int ks = 0; ks < G::KS; ++ks) {
+      if ((ks & (WARPS - 1)) != warp) continue;
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = x[4 * ks + i] * f0 * f1;
+      const uint2 hi = make_uint2(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]));
+      qf[(n * G::PARTS * G::KS + ks) * 32] = hi;
+      if constexpr (G::PARTS == 2) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+        qf[((n * G::PARTS + 1) * G::KS + ks) * 32] =
+            make_uint2(pack_half2((y[0] - a.x) * 2048.f, (y[1] - a.y) * 2048.f),
+                       pack_half2((y[2] - b.x) * 2048.f, (y[3] - b.y) * 2048.f));
+      }
     }
-    if (lane == 0) hs[h] = p.scale_log2 * __int_as_float((127 + e0) << 23) * __int_as_float((127 + e1) << 23);
   }
   __syncthreads();
-  const uint2* qf = reinterpret_cast<const uint2*>(smem + G::Q_OFF) + lane;
-  uint2 qr[G::Q_REGS ? NT * G::PARTS * G::KS : 1];
-  if constexpr (G::Q_REGS)
-#pragma unroll
-    for (int i = 0; i < NT * G::PARTS * G::KS; ++i) qr[i] = qf[i * 32];
 
-  // This lane's columns are heads 8 n + 2 tl and + 1 of each N tile n.
-  // ms and mos are the maxima as exponents are taken against them (safe_max).
-  float fs[NT][2], m[NT][2], mo[NT][2], ms[NT][2], mos[NT][2], l[NT][2], acc[NT][G::KS][4];
+  // This lane's columns are heads 8 n + 2 tl and + 1 of each N tile n. ms and mos are the maxima as exponents are taken
+  // against them (safe_max).
+  float m[NT][2], mo[NT][2], ms[NT][2], mos[NT][2], l[NT][2], acc[NT][G::KS][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      fs[n][c] = hs[8 * n + 2 * tl + c];
       m[n][c] = mo[n][c] = -INFINITY;
       ms[n][c] = mos[n][c] = l[n][c] = 0.f;
     }
@@ -407,26 +539,32 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
     for (int i = 0; i < G::KS; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
   }
 
-  for (int j = 0; j < my_n; ++j) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 1) : "memory");
-    __syncwarp();   // the other lanes' scales
-    const uint8_t* slot = ring + (j % G::STAGES) * G::SLOT;
-    const float* sc = reinterpret_cast<const float*>(slot + G::S_OFF);
-    const int k0 = (warp + WARPS * j) * TILE;
-    float s[NT][4];
-    {
-      // two chains of products, so that one's latency covers the other's
-      float a[NT][G::PARTS][2][4];
+  int late = 0;   // 1, 2: K, V did not come in time
+  int j = 0;
+  for (; j < my_n; ++j) {
+    const float ks_mine = ks_next, vs_mine = vs_next;
+    if (j % SEG == SEG / 2 - 1 && j + SEG / 2 + 1 < my_n) look_up(j / SEG + 1);
+    if (j + 1 < my_n) load_scales(j + 1);
+    if (!wait(kbar, j)) {
+      late = 1;
+      break;
+    }
+    const uint8_t* kbuf = buf + (j % G::STAGES) * G::STEP_BYTES;
+    const uint8_t* vbuf = buf + (G::STAGES + j % G::STAGES) * G::STEP_BYTES;
+    float s[2][NT][4];   // keys 16 t + gl (c 0, 1) and + 8 (c 2, 3)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      float a[NT][G::PARTS][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int q = 0; q < G::PARTS; ++q)
-#pragma unroll
-          for (int c = 0; c < 8; ++c) a[n][q][c >> 2][c & 3] = 0.f;
+        for (int q = 0; q < G::PARTS; ++q) a[n][q][0] = a[n][q][1] = a[n][q][2] = a[n][q][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < G::KC; ++c) {
-        const uint4 u = *reinterpret_cast<const uint4*>(slot + c * 512 + lane * 16);
-        const uint4 w = *reinterpret_cast<const uint4*>(slot + (G::KC + c) * 512 + lane * 16);
+        const int a0_at = WHOLE ? G::box_at(t * TILE + gl, k_chunk<HD>(tl, c)) : ((2 * t * G::KC + c) * 32 + lane) * 16;
+        const int a1_at = WHOLE ? G::box_at(t * TILE + gl + 8, k_chunk<HD>(tl, c)) : a0_at + G::KC * 512;
+        const uint4 u = *reinterpret_cast<const uint4*>(kbuf + a0_at);
+        const uint4 w = *reinterpret_cast<const uint4*>(kbuf + a1_at);
         const uint32_t ku[4] = {u.x, u.y, u.z, u.w}, kw[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -435,9 +573,8 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int q = 0; q < G::PARTS; ++q) {
-              const int at_q = (n * G::PARTS + q) * G::KS + c * 4 + i;
-              const uint2 b = G::Q_REGS ? qr[G::Q_REGS ? at_q : 0] : qf[at_q * 32];
-              mma_f16(a[n][q][i & 1], a0, a1, a2, a3, b.x, b.y);
+              const uint2 b = qf[((n * G::PARTS + q) * G::KS + c * 4 + i) * 32];
+              mma_f16(a[n][q], a0, a1, a2, a3, b.x, b.y);
             }
         }
       }
@@ -445,105 +582,154 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          s[n][c] = a[n][0][0][c] + a[n][0][1][c];
-          if constexpr (G::PARTS == 2) s[n][c] = fmaf(a[n][1][0][c] + a[n][1][1][c], 1.f / 2048.f, s[n][c]);
+          s[t][n][c] = a[n][0][c];
+          if constexpr (G::PARTS == 2) s[t][n][c] = fmaf(a[n][1][c], 1.f / 2048.f, s[t][n][c]);
         }
     }
-    // Scores of keys gl (c 0, 1) and gl + 8 (c 2, 3), log2 domain; u: with the exponent of the value's scale.
-    const bool in0 = k0 + gl < n_keys, in1 = k0 + gl + 8 < n_keys;
-    float e[2], mant[2];
-    split_scale(sc[TILE + gl], e[0], mant[0]);
-    split_scale(sc[TILE + gl + 8], e[1], mant[1]);
-    const float ks[2] = {sc[gl], sc[gl + 8]};
+    __syncwarp();
+    if (j + G::STAGES < my_n) issue_k(j + G::STAGES);   // over the K just read
+    commit();
+
+    // Scores in the log2 domain; e: the exponent (fp32: its whole part) of the value's scale.
+    float e_mine, mant_mine = 1.f;
+    if constexpr (G::PARTS == 2)
+      split_scale(vs_mine, e_mine, mant_mine);
+    else
+      e_mine = lg2(vs_mine);
+    float e[2][2], mant[2][2];
+    const int left = n_keys - (warp + WARPS * j) * STEP;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int key = t * TILE + 8 * k + gl;
+        const float ks = __shfl_sync(0xffffffffu, ks_mine, key);
+        e[t][k] = __shfl_sync(0xffffffffu, e_mine, key);
+        if constexpr (G::PARTS == 2) mant[t][k] = __shfl_sync(0xffffffffu, mant_mine, key);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            s[t][n][2 * k + c] *= fs[n][c] * ks;
+            if (left < STEP && key >= left) s[t][n][2 * k + c] = -INFINITY;
+          }
+      }
     bool raise = false;
+    float tm[NT][2], tmo[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[n][c] = (c < 2 ? in0 : in1) ? s[n][c] * (fs[n][c & 1] * ks[c >> 1]) : -INFINITY;
-        raise |= s[n][c] > m[n][c & 1] + SLACK || s[n][c] + e[c >> 1] > mo[n][c & 1] + SLACK;
+      for (int c = 0; c < 2; ++c) {
+        tm[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
+        tmo[n][c] = fmaxf(fmaxf(s[0][n][c] + e[0][0], s[0][n][c + 2] + e[0][1]),
+                          fmaxf(s[1][n][c] + e[1][0], s[1][n][c + 2] + e[1][1]));
+        raise |= tm[n][c] > m[n][c] + SLACK || tmo[n][c] > mo[n][c] + SLACK;
       }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float t = fmaxf(s[n][c], s[n][c + 2]), u = fmaxf(s[n][c] + e[0], s[n][c + 2] + e[1]);
+          float x = tm[n][c], y = tmo[n][c];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-            u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, o));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
           }
-          t = fmaxf(t, m[n][c]);
-          u = fmaxf(u, mo[n][c]);
-          ms[n][c] = safe_max(t);
-          mos[n][c] = safe_max(u);
-          const float cl = ex2(m[n][c] - ms[n][c]), co = ex2(mo[n][c] - mos[n][c]);
-          l[n][c] *= cl;
+          x = fmaxf(x, m[n][c]);
+          y = fmaxf(y, mo[n][c]);
+          ms[n][c] = safe_max(x);
+          mos[n][c] = safe_max(y);
+          const float co = ex2(mo[n][c] - mos[n][c]);
+          l[n][c] *= ex2(m[n][c] - ms[n][c]);
 #pragma unroll
           for (int i = 0; i < G::KS; ++i) {
             acc[n][i][c] *= co;
             acc[n][i][c + 2] *= co;
           }
-          m[n][c] = t;
-          mo[n][c] = u;
+          m[n][c] = x;
+          mo[n][c] = y;
         }
     }
-    uint32_t pb[NT][G::PARTS][2];
+    uint32_t pb[2][NT][G::PARTS][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float w[4];
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const bool in = c < 2 ? in0 : in1;
-        l[n][c & 1] += in ? ex2(s[n][c] - ms[n][c & 1]) : 0.f;
-        w[c] = in ? ex2(s[n][c] + e[c >> 1] - mos[n][c & 1]) * mant[c >> 1] : 0.f;
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          l[n][c & 1] += ex2(s[t][n][c] - ms[n][c & 1]);
+          w[c] = ex2(s[t][n][c] + e[t][c >> 1] - mos[n][c & 1]);
+          if constexpr (G::PARTS == 2) w[c] *= mant[t][c >> 1];
+        }
+        const uint32_t p0 = pack_half2(w[0], w[1]), p1 = pack_half2(w[2], w[3]);
+        pb[t][n][0][0] = movmatrix_trans(p0);
+        pb[t][n][0][1] = movmatrix_trans(p1);
+        if constexpr (G::PARTS == 2) {
+          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&p0));
+          const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&p1));
+          pb[t][n][1][0] = movmatrix_trans(pack_half2(w[0] - f0.x, w[1] - f0.y));
+          pb[t][n][1][1] = movmatrix_trans(pack_half2(w[2] - f1.x, w[3] - f1.y));
+        }
       }
-      const uint32_t p0 = pack_half2(w[0], w[1]), p1 = pack_half2(w[2], w[3]);
-      pb[n][0][0] = movmatrix_trans(p0);
-      pb[n][0][1] = movmatrix_trans(p1);
-      if constexpr (G::PARTS == 2) {
-        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&p0));
-        const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&p1));
-        pb[n][1][0] = movmatrix_trans(pack_half2(w[0] - f0.x, w[1] - f0.y));
-        pb[n][1][1] = movmatrix_trans(pack_half2(w[2] - f1.x, w[3] - f1.y));
-      }
+    if (!wait(vbar, j)) {
+      late = 2;
+      break;
     }
     // V: words of four dims of this lane's four keys, paired by key.
-    const uint8_t* vs = slot + G::V_OFF + lane * G::VB;
 #pragma unroll
-    for (int c = 0; c < G::VC; ++c) {
-      uint32_t v[4][G::VB / 4];
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* src = vs + (i * G::VC + c) * 32 * G::VB;
-        if constexpr (G::VB == 16) {
-          const uint4 u = *reinterpret_cast<const uint4*>(src);
-          v[i][0] = u.x, v[i][1] = u.y, v[i][2] = u.z, v[i][3] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(src);
-          v[i][0] = u.x, v[i][1] = u.y;
+      for (int c = 0; c < G::VC; ++c) {
+        uint32_t v[4][G::VB / 4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = t * TILE + 2 * tl + (i & 1) + 4 * (i & 2);
+          const int v_at = !WHOLE ? (((t * 4 + i) * G::VC + c) * 32 + lane) * G::VB
+                                  : HD == 64 ? G::box_at(row, gl >> 1) + (gl & 1) * 8 : G::box_at(row, c * 8 + gl);
+          const uint8_t* src = vbuf + v_at;
+          if constexpr (G::VB == 16) {
+            const uint4 u = *reinterpret_cast<const uint4*>(src);
+            v[i][0] = u.x, v[i][1] = u.y, v[i][2] = u.z, v[i][3] = u.w;
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(src);
+            v[i][0] = u.x, v[i][1] = u.y;
+          }
+          if (WHOLE && left < STEP && row >= left) {   // whatever lies behind the last visible key, NaN codes too
+#pragma unroll
+            for (int w = 0; w < G::VB / 4; ++w) v[i][w] = 0;
+          }
         }
+#pragma unroll
+        for (int w = 0; w < G::VB / 4; ++w)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7362u : 0x5140u;
+            const uint32_t x = __byte_perm(v[0][w], v[1][w], sel), y = __byte_perm(v[2][w], v[3][w], sel);
+            const uint32_t a0 = lo_pair(x), a1 = hi_pair(x), a2 = lo_pair(y), a3 = hi_pair(y);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int q = 0; q < G::PARTS; ++q)
+                mma_f16(acc[n][(c * (G::VB / 4) + w) * 2 + half], a0, a1, a2, a3, pb[t][n][q][0], pb[t][n][q][1]);
+          }
       }
-#pragma unroll
-      for (int w = 0; w < G::VB / 4; ++w)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t sel = half ? 0x7362u : 0x5140u;
-          const uint32_t x = __byte_perm(v[0][w], v[1][w], sel), y = __byte_perm(v[2][w], v[3][w], sel);
-          const uint32_t a0 = lo_pair(x), a1 = hi_pair(x), a2 = lo_pair(y), a3 = hi_pair(y);
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int q = 0; q < G::PARTS; ++q)
-              mma_f16(acc[n][(c * (G::VB / 4) + w) * 2 + half], a0, a1, a2, a3, pb[n][q][0], pb[n][q][1]);
-        }
-    }
-    __syncwarp();   // every lane has read the slot's scales
-    if (j + G::STAGES < my_n) issue(j + G::STAGES);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    __syncwarp();
+    if (j + G::STAGES < my_n) issue_v(j + G::STAGES);
+    commit();
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if constexpr (WHOLE) {
+    if (late) {   // let the copies in flight land (bounded) before the shared memory is given back or used again
+      const int k0 = late == 1 ? j : j + 1;   // K of step j is in use already where V did not come
+      for (int k = k0; k < k0 + G::STAGES && k < my_n; ++k)
+        mbar_wait(&kbar[k % G::STAGES], static_cast<uint32_t>((k / G::STAGES) & 1), p.err);
+      for (int k = j; k < j + G::STAGES && k < my_n; ++k)
+        mbar_wait(&vbar[k % G::STAGES], static_cast<uint32_t>((k / G::STAGES) & 1), p.err);
+    }
+  } else {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
 
   // Merge the warps: sums against max m, through shared memory.
 #pragma unroll
@@ -552,9 +738,10 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], o);
-  __syncthreads();   // ring, q and offsets are free
+  if (__syncthreads_or(late)) return;   // buffers, q and offsets are free; a CTA that gave up leaves no result
   float* osm = reinterpret_cast<float*>(smem);                     // [WARPS][8 NT][O_ROW]
   float* msm = osm + WARPS * 8 * NT * G::O_ROW;                    // [WARPS][8 NT][2]
+  float* wsm = msm + WARPS * 8 * NT * 2;                           // [8 NT][WARPS]
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -563,7 +750,7 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
       const float f = exp2f(mos[n][c] - ms[n][c]);
 #pragma unroll
       for (int i = 0; i < G::KS; ++i)
-        *reinterpret_cast<float2*>(osm + h * G::O_ROW + gl * (HD / 8) + 2 * i) =
+        *reinterpret_cast<float2*>(osm + h * G::O_ROW + i / (G::VB / 2) * 128 + gl * G::VB + 2 * (i % (G::VB / 2))) =
             make_float2(acc[n][i][c] * f, acc[n][i][c + 2] * f);
       if (gl == 0) {
         msm[2 * h] = m[n][c];
@@ -571,28 +758,46 @@ __global__ void __launch_bounds__(32 * WARPS) quant_decode_tc_kernel(Params p) {
       }
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < heads * HD; i += blockDim.x) {
-    const int h = i / HD, d = i % HD;
-    float top = -INFINITY, total = 0.f, o = 0.f;
+  const int64_t part0 = (r * p.nh + kvh * p.rep + h0) * p.splits + split;   // head h: part0 + h * splits
+  for (int h = threadIdx.x; h < heads; h += blockDim.x) {
+    float top = -INFINITY, total = 0.f, f[WARPS];
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) top = fmaxf(top, msm[2 * (w * 8 * NT + h)]);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      const float f = exp2f(msm[2 * (w * 8 * NT + h)] - safe_max(top));
-      total += f * msm[2 * (w * 8 * NT + h) + 1];
-      o += f * osm[(w * 8 * NT + h) * G::O_ROW + d];
+      f[w] = ex2(msm[2 * (w * 8 * NT + h)] - safe_max(top));
+      total += f[w] * msm[2 * (w * 8 * NT + h) + 1];
     }
-    const int hh = kvh * p.rep + h0 + h;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) wsm[h * WARPS + w] = p.splits == 1 ? f[w] / total : f[w];
+    if (p.splits > 1) {
+      float* ml = p.ws + static_cast<int64_t>(gridDim.z) * p.nh * p.splits * HD +
+                  2 * (part0 + static_cast<int64_t>(h) * p.splits);
+      ml[0] = top;
+      ml[1] = total;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x * 4; i < heads * HD; i += blockDim.x * 4) {
+    const int h = i / HD, d = i % HD;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float4 x = *reinterpret_cast<const float4*>(osm + (w * 8 * NT + h) * G::O_ROW + d);
+      const float f = wsm[h * WARPS + w];
+      o.x = fmaf(f, x.x, o.x);
+      o.y = fmaf(f, x.y, o.y);
+      o.z = fmaf(f, x.z, o.z);
+      o.w = fmaf(f, x.w, o.w);
+    }
     if (p.splits == 1) {
-      static_cast<T*>(p.out)[r * p.ldo + static_cast<int64_t>(hh) * HD + d] = from_f<T>(o / total);
+      T* dst = static_cast<T*>(p.out) + r * p.ldo + static_cast<int64_t>(kvh * p.rep + h0 + h) * HD + d;
+      dst[0] = from_f<T>(o.x);
+      dst[1] = from_f<T>(o.y);
+      dst[2] = from_f<T>(o.z);
+      dst[3] = from_f<T>(o.w);
     } else {
-      const int64_t part = (r * p.nh + hh) * p.splits + split;
-      p.ws[part * HD + d] = o;
-      if (d == 0) {
-        float* ml = p.ws + static_cast<int64_t>(gridDim.z) * p.nh * p.splits * HD + 2 * part;
-        ml[0] = top;
-        ml[1] = total;
-      }
+      *reinterpret_cast<float4*>(p.ws + (part0 + static_cast<int64_t>(h) * p.splits) * HD + d) = o;
     }
   }
 }
@@ -603,11 +808,26 @@ bool supported(const Params& p) {
          ((reinterpret_cast<uintptr_t>(p.kv.k) | reinterpret_cast<uintptr_t>(p.kv.v)) & 15) == 0;
 }
 
+// Tensor maps see the cache as rows of hd bytes: whole rows between heads and blocks, and 31-bit row numbers.
+bool whole_tiles(const Params& p) {
+  if (p.kv.block_size % TILE || p.kv.block_stride % p.hd || p.kv.head_stride % p.hd) return false;
+  if (p.kv.head_stride < 0 || p.kv.block_stride < 0) return false;
+  return (p.kv.num_blocks - 1) * (p.kv.block_stride / p.hd) + (p.nkv - 1) * (p.kv.head_stride / p.hd) +
+             p.kv.block_size <= INT32_MAX - 2 * TILE;
+}
+
 template <typename T, int HD, int NT, bool WHOLE>
 int launch_geo(Params p, int64_t B, int64_t nkv, cudaStream_t st) {
   using G = Geo<T, HD, NT, WHOLE>;
   p.groups = (p.rep + 8 * NT - 1) / (8 * NT);
   if (nkv * p.groups > 65535) return fail("fs_attention_decode_quant: too many heads");
+  CUtensorMap mk = {}, mv = {};
+  if constexpr (WHOLE) {
+    p.rows_per_block = static_cast<int>(p.kv.block_stride / HD);
+    p.rows_per_head = static_cast<int>(p.kv.head_stride / HD);
+    p.map_rows = static_cast<int>((p.kv.num_blocks - 1) * p.rows_per_block + (nkv - 1) * p.rows_per_head + p.kv.block_size);
+    if (make_byte_map(&mk, p.kv.k, HD, p.map_rows, TILE) || make_byte_map(&mv, p.kv.v, HD, p.map_rows, TILE)) return -1;
+  }
   static bool attr[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -618,13 +838,13 @@ int launch_geo(Params p, int64_t B, int64_t nkv, cudaStream_t st) {
     attr[dev] = true;
   }
   const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(nkv * p.groups), static_cast<unsigned>(B));
-  launch_pdl_async(quant_decode_tc_kernel<T, HD, NT, WHOLE>, grid, 32 * WARPS, G::SMEM, st, p);
+  launch_pdl_async(quant_decode_tc_kernel<T, HD, NT, WHOLE>, grid, 32 * WARPS, G::SMEM, st, mk, mv, p);
   return check_launch("quant_decode_tc_kernel");
 }
 
 template <typename T, int HD>
 int launch_hd(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
-  const bool whole = p.kv.block_size % TILE == 0;
+  const bool whole = whole_tiles(p);
   if (p.rep > 8)   // two N tiles read the cache once for up to 16 heads
     return whole ? launch_geo<T, HD, 2, true>(p, B, nkv, st) : launch_geo<T, HD, 2, false>(p, B, nkv, st);
   return whole ? launch_geo<T, HD, 1, true>(p, B, nkv, st) : launch_geo<T, HD, 1, false>(p, B, nkv, st);
@@ -638,46 +858,63 @@ int launch_t(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
 
 }  // namespace tc
 
-// Joins the splits of a (row, head), weights exp2(m_split - m): four warps take the splits in turn, lanes the dims.
+// Joins the splits of a (row, head): weights exp2(m_split - m) to shared memory, then the threads take two dims each of
+// every GROUPS-th split, GROUPS = 128 / (hd / 2, rounded up to a power of two).
+constexpr int MAX_SPLITS = ONE_WAVE;
 template <typename T>
 __global__ void __launch_bounds__(128) quant_combine_kernel(Params p) {
   pdl_trigger();
   pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
-  constexpr int MAXD = 8;
-  __shared__ float red[4], sums[4], part[4][32 * MAXD];
+  __shared__ float w[MAX_SPLITS], red[8];
+  __shared__ float2 sums[128];
   const int64_t r = blockIdx.y;
-  const int h = blockIdx.x, hd = p.hd, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t n_vis = visible(p, r), base = (r * p.nh + h) * p.splits;
-  const int used = static_cast<int>((n_vis + SPLIT_KEYS - 1) / SPLIT_KEYS);
-  const float* ml = p.ws + static_cast<int64_t>(gridDim.y) * p.nh * p.splits * hd + 2 * base;
-  const float* o = p.ws + base * hd;
+  const int h = blockIdx.x, hd = p.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t n_vis = visible(p, r), base = (r * p.nh + h) * p.splits, per = split_keys(n_vis, p.nkv);
+  const int used = static_cast<int>((n_vis + per - 1) / per);
+  const float2* ml = reinterpret_cast<const float2*>(p.ws + static_cast<int64_t>(gridDim.y) * p.nh * p.splits * hd) + base;
   float top = -INFINITY;
-  for (int s = threadIdx.x; s < used; s += blockDim.x) top = fmaxf(top, ml[2 * s]);
+  for (int s = tid; s < used; s += 128) {
+    w[s] = ml[s].x;
+    top = fmaxf(top, w[s]);
+  }
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
   if (lane == 0) red[warp] = top;
   __syncthreads();
   top = safe_max(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-  float total = 0.f, acc[MAXD];
-#pragma unroll
-  for (int i = 0; i < MAXD; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int s = warp; s < used; s += 4) {
-    const float2 v = *reinterpret_cast<const float2*>(ml + 2 * s);
-    const float w = exp2f(v.x - top);
-    total += w * v.y;
-#pragma unroll
-    for (int i = 0; i < MAXD; ++i)
-      if (lane + 32 * i < hd) acc[i] = fmaf(w, o[static_cast<int64_t>(s) * hd + lane + 32 * i], acc[i]);
+  float total = 0.f;
+  for (int s = tid; s < used; s += 128) {
+    w[s] = exp2f(w[s] - top);
+    total += w[s] * ml[s].y;
   }
-  if (lane == 0) sums[warp] = total;
 #pragma unroll
-  for (int i = 0; i < MAXD; ++i) part[warp][lane + 32 * i] = acc[i];
+  for (int i = 16; i > 0; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
+  if (lane == 0) red[4 + warp] = total;
   __syncthreads();
-  total = sums[0] + sums[1] + sums[2] + sums[3];
-  for (int d = threadIdx.x; d < hd; d += blockDim.x)
-    static_cast<T*>(p.out)[r * p.ldo + static_cast<int64_t>(h) * hd + d] =
-        from_f<T>(n_vis == 0 ? 0.f : (part[0][d] + part[1][d] + part[2][d] + part[3][d]) / total);
+  total = red[4] + red[5] + red[6] + red[7];
+  const int cols = hd / 2, width = cols <= 1 ? 1 : 1 << (32 - __clz(cols - 1)), groups = 128 / width;
+  const int col = tid & (width - 1), group = tid / width;
+  float2 o = make_float2(0.f, 0.f);
+  if (col < cols) {
+    const float2* src = reinterpret_cast<const float2*>(p.ws + base * hd) + col;
+#pragma unroll 8
+    for (int s = group; s < used; s += groups) {
+      const float2 x = src[static_cast<int64_t>(s) * cols];
+      o.x = fmaf(w[s], x.x, o.x);
+      o.y = fmaf(w[s], x.y, o.y);
+    }
+  }
+  sums[tid] = o;
+  __syncthreads();
+  if (tid < cols) {
+    for (int g = 1; g < groups; ++g) {
+      o.x += sums[g * width + tid].x;
+      o.y += sums[g * width + tid].y;
+    }
+    T* dst = static_cast<T*>(p.out) + r * p.ldo + static_cast<int64_t>(h) * hd + 2 * tid;
+    dst[0] = from_f<T>(n_vis == 0 ? 0.f : o.x / total);
+    dst[1] = from_f<T>(n_vis == 0 ? 0.f : o.y / total);
+  }
 }
 
 template <typename T>
@@ -707,10 +944,14 @@ int launch_t(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
 
 }  // namespace
 
-int64_t splits(int64_t n_slots) { return (n_slots + SPLIT_KEYS - 1) / SPLIT_KEYS; }
+// Most splits that any row of up to n_slots visible slots has (split_keys): the grid and the workspace are made for it.
+int64_t splits(int64_t nkv, int64_t n_slots) {
+  const int64_t units = (n_slots + UNIT_KEYS - 1) / UNIT_KEYS, most = (ONE_WAVE + nkv - 1) / nkv;
+  return units < most ? units : most;
+}
 
-int64_t workspace_bytes(int64_t B, int64_t nh, int64_t hd, int64_t n_slots) {
-  const int64_t s = splits(n_slots);
+int64_t workspace_bytes(int64_t B, int64_t nh, int64_t nkv, int64_t hd, int64_t n_slots) {
+  const int64_t s = splits(nkv, n_slots);
   return s <= 1 ? 0 : B * nh * s * (hd + 2) * static_cast<int64_t>(sizeof(float));
 }
 
@@ -729,8 +970,10 @@ int launch(int dtype, const void* q, int64_t ldq, const KVCache& kv, const KVSca
   p.nh = static_cast<int>(nh);
   p.rep = static_cast<int>(nh / nkv);
   p.hd = static_cast<int>(hd);
-  p.splits = static_cast<int>(splits(n_slots));
+  p.nkv = static_cast<int>(nkv);
+  p.splits = static_cast<int>(splits(nkv, n_slots));
   p.groups = (p.rep + HEADS - 1) / HEADS;
+  p.q_vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ldq % (dtype == F32 ? 4 : 8) == 0;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.ws = ws;
   p.err = error_word();

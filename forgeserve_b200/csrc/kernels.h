@@ -70,8 +70,7 @@ int kv_dequant(int dtype, const KVCache& kv, const KVScales& sc, int64_t B, int6
                void* k_out, void* v_out, cudaStream_t st);
 
 namespace decode_quant {   // attention_decode_quant.cu
-int64_t splits(int64_t n_slots);
-int64_t workspace_bytes(int64_t B, int64_t nh, int64_t hd, int64_t n_slots);
+int64_t workspace_bytes(int64_t B, int64_t nh, int64_t nkv, int64_t hd, int64_t n_slots);
 int launch(int dtype, const void* q, int64_t ldq, const KVCache& kv, const KVScales& sc, int64_t n_slots,
            const int64_t* positions, void* out, int64_t ldo, int64_t B, int64_t nh, int64_t nkv, int64_t hd, float scale,
            float* ws, cudaStream_t st);

@@ -356,7 +356,7 @@ def attention_decode_quant(q: torch.Tensor, kv: L.KVQuantDesc, n_slots: int, pos
     _check_positions(positions, B)
     _check_cache(kv, B, nkv, hd, dev, torch.float8_e4m3fn)
     lib = L.load()
-    need = lib.fs_attention_decode_quant_workspace(B, nh, hd, n_slots)
+    need = lib.fs_attention_decode_quant_workspace(B, nh, nkv, hd, n_slots)
     # Allocated by each call: the allocator hands it out in stream order, and a captured call's stays with its graph.
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     with torch.cuda.device(dev):

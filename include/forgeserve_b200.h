@@ -212,7 +212,7 @@ int fs_kv_dequant(const fs_kv_quant* kv, int64_t B, int64_t n_slots, int64_t nkv
 /* fs_attention_decode over an 8-bit cache: one query a row, any n_heads / n_kv_heads, head_dim even and <= 256. A row
  * with a negative position sees no slot and gets zeros. workspace: fs_attention_decode_quant_workspace(...) bytes (0 up
  * to 512 slots), 16-byte aligned, as for fs_attention_decode. */
-int64_t fs_attention_decode_quant_workspace(int64_t B, int64_t nh, int64_t hd, int64_t n_slots);
+int64_t fs_attention_decode_quant_workspace(int64_t B, int64_t nh, int64_t nkv, int64_t hd, int64_t n_slots);
 int fs_attention_decode_quant(const void* q, int64_t ldq, const fs_kv_quant* kv, int64_t n_slots,
                               const int64_t* positions, void* out, int64_t ldo, int64_t B, int64_t nh, int64_t nkv,
                               int64_t hd, float scale, void* workspace, int64_t workspace_bytes, int dtype,

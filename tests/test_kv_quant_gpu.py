@@ -339,6 +339,11 @@ DECODE_CASES = [  # dtype, lengths, nh, nkv, hd, bs
     (torch.float32, [640, 30], 9, 1, 256, 48),
     (torch.float32, [640, 30], 4, 2, 96, 16),
     (torch.float32, [70], 3, 3, 6, 2),
+    # rows long enough for splits of several units of 512 slots, beside short ones
+    (torch.bfloat16, [19000, 700, 9500, 4700], 64, 64, 64, 16),
+    (torch.bfloat16, [11000, 513, 5000], 256, 128, 128, 24),
+    (torch.float32, [6000, 40], 200, 200, 64, 16),
+    (torch.bfloat16, [6000, 3100], 100, 100, 32, 16),
 ]
 
 

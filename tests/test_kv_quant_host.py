@@ -175,8 +175,8 @@ def test_dequant_and_decode_refusals(lib):
                      (dict(dtype=9), b"dtype"), (dict(B=70000), b"too many")):
         assert dec(**kw) == -1 and word in lib.fs_last_error(), (kw, lib.fs_last_error())
     long = quant_desc(table_cols=64, table_stride=64)
-    need = lib.fs_attention_decode_quant_workspace(1, 4, 128, 1024)
-    assert need == 4 * 2 * 130 * 4 and lib.fs_attention_decode_quant_workspace(1, 4, 128, 512) == 0
+    need = lib.fs_attention_decode_quant_workspace(1, 4, 2, 128, 1024)
+    assert need == 4 * 2 * 130 * 4 and lib.fs_attention_decode_quant_workspace(1, 4, 2, 128, 512) == 0
     for kw in (dict(), dict(ws=P, wsb=need - 1), dict(ws=ctypes.c_void_p(4097), wsb=need)):
         assert dec(kv=ctypes.byref(long), n=1024, **kw) == -1 and b"workspace" in lib.fs_last_error()
     assert dec(B=0) == 0
