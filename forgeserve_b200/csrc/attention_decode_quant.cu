@@ -25,7 +25,8 @@ namespace decode_quant {
 
 namespace {
 
-constexpr int UNIT_KEYS = 512;   // a split is a multiple of this
+constexpr int UNIT_KEYS = 512;   // a split is a multiple of this (256 took 97 us on the 64 rows below, 1024 77, but
+                                 // 16 us on one row of 4096 slots instead of 12)
 constexpr int ONE_WAVE = 592;    // CTAs that run at once: 4 on each of 148 SMs
 constexpr int HEADS = 8;         // query heads of one KV head that a CTA of the general kernel handles
 
@@ -47,7 +48,7 @@ struct Params {
   const int64_t* positions;
   void* out;
   int64_t ldo;
-  int nh, nkv, rep, hd, splits, groups;   // groups: CTAs a KV head, of HEADS (or 8 NT) query heads each
+  int B, nh, nkv, rep, hd, splits, groups;   // groups: CTAs a KV head, of HEADS (or 8 NT) query heads each
   bool q_vec;                        // rows of q on 16-byte boundaries
   int rows_per_block, rows_per_head, map_rows;   // of the tensor maps' hd-wide rows (WHOLE)
   float scale_log2;
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
 //     S^T (16 keys x 8 heads) = K (16 x hd) Q^T (hd x 8),   O^T (hd x 8 heads) += V^T (hd x 16) P^T (16 x 8)
 // A contraction's index order is free as long as both operands agree, and so are the rows of O^T; they are chosen so
 // that every lane's operand values are neighbouring bytes of a cache row: lane (g, t) = (lane / 4, lane % 4) takes, of
-// keys g and g + 8, the 16-byte chunks 2t and 2t + 1 of each 128 bytes for K, and of keys 2t, 2t+1, 2t+8, 2t+9 the chunk
+// keys g and g + 8, two 16-byte chunks of each 128 bytes for K (k_chunk), and of keys 2t, 2t+1, 2t+8, 2t+9 the chunk
 // g for V (8 bytes of it at hd 64). P^T reaches the B layout by movmatrix.
 //
 // A warp takes STEP keys at a time, into a ring of its own; no barrier joins the warps before the end.
@@ -191,18 +192,9 @@ __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
 // vote a step instead of a reduction.
 namespace tc {
 
-#ifndef NWARPS
-#define NWARPS 4
-#endif
-#ifndef NSTAGES
-#define NSTAGES 1
-#endif
-#ifndef MINB
-#define MINB 4
-#endif
-constexpr int WARPS = NWARPS, TILE = 16, STEP = 32;   // a warp takes STEP keys (two tiles) at a time
-constexpr int SEG = UNIT_KEYS / STEP / WARPS;         // steps whose places a warp looks up at once
-constexpr float SLACK = 8.f;
+constexpr int WARPS = 4, TILE = 16, STEP = 32;   // a warp takes STEP keys (two tiles) at a time
+constexpr int SEG = 4;         // steps whose places a warp looks up at once
+constexpr float SLACK = 8.f, LOWEST = -3e38f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -258,31 +250,24 @@ __device__ __forceinline__ float lg2(float x) {
   return y;
 }
 
-// 16 neighbouring values as fp32, by 16-byte loads where `vec`.
-__device__ __forceinline__ void load16(const __nv_bfloat16* q, bool vec, float* x) {
+// 16 neighbouring values, by 16-byte loads where `vec`: two bf16 a word (8 words), or fp32 (16 words).
+__device__ __forceinline__ void load16(const __nv_bfloat16* q, bool vec, uint32_t* x) {
   if (vec) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 u = *reinterpret_cast<const uint4*>(q + 8 * i);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-        x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-      }
-    }
+    *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(q);
+    *reinterpret_cast<uint4*>(x + 4) = *reinterpret_cast<const uint4*>(q + 8);
   } else {
+    const uint16_t* u = reinterpret_cast<const uint16_t*>(q);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = to_f(q[i]);
+    for (int i = 0; i < 8; ++i) x[i] = u[2 * i] | static_cast<uint32_t>(u[2 * i + 1]) << 16;
   }
 }
-__device__ __forceinline__ void load16(const float* q, bool vec, float* x) {
+__device__ __forceinline__ void load16(const float* q, bool vec, uint32_t* x) {
   if (vec) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(x + 4 * i) = *reinterpret_cast<const float4*>(q + 4 * i);
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(x + 4 * i) = *reinterpret_cast<const uint4*>(q + 4 * i);
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = q[i];
+    for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(q[i]);
   }
 }
 
@@ -308,7 +293,9 @@ struct Geo {
   static constexpr int BOX = HD < 128 ? 64 : 128;             // bytes of a box's row
   static constexpr int BOXES = HD / BOX;                      // boxes a row
   static constexpr int STEP_BYTES = STEP * HD;                // K (or V) of a step
-  static constexpr int STAGES = WHOLE ? NSTAGES : 1;
+  // One step deep: K of the next step is on its way from the scores on, its V from the V product on. Two steps take the
+  // shared memory of a fourth CTA an SM (64 rows: 89 us against 80).
+  static constexpr int STAGES = 1;
   static constexpr int BUF = 2 * STAGES * STEP_BYTES;         // a warp's ring: K stages, then V stages
   static constexpr int Q_OFF = WARPS * BUF;                   // q as B operands: [NT][PARTS][KS][32 lanes] of 8 bytes
   static constexpr int AT_OFF = Q_OFF + NT * PARTS * KS * 256;   // where tiles or keys lie: [2][values, scales][WARPS][LOOK]
@@ -318,7 +305,10 @@ struct Geo {
   static constexpr int O_ROW = HD + 4;                        // padded: the lanes' writes spread over the banks
   static constexpr int O_BYTES = WARPS * 8 * NT * (O_ROW + 3) * 4;   // the warps' sums, (max, sum), weights, over all that
   static constexpr int SMEM = (O_BYTES > END ? O_BYTES : END) + (WHOLE ? 1024 : 0);   // boxes lie on 1024 bytes
-  static constexpr int CTAS = NT == 1 && HD <= 128 ? MINB : 1;   // an SM (registers)
+  // CTAs an SM that the registers are held to: the most that spill little (hd 128: 80 us on 64 rows at 4, 87 at 3; 16 heads
+  // a KV head 65 at 3, 76 unbounded; hd 64, MHA 50 at 6, 55 at 4; hd 256 31 at 3, 34 unbounded).
+  static constexpr int CTAS = NT == 1 ? (HD == 64 ? (sizeof(T) == 2 ? 6 : 5) : HD == 128 ? 4 : 3)
+                                      : (HD == 64 ? 4 : HD == 128 ? 3 : 2);
   // byte of a K (or V) step's 16-byte chunk `chunk` of row `row`
   static __device__ __forceinline__ int box_at(int row, int chunk) {
     const int tile = row >> 4, r = row & 15;
@@ -326,10 +316,11 @@ struct Geo {
     return tile * 16 * HD + (chunk >> 3) * 16 * 128 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
   }
 };
-// The 16-byte chunk of a K row that lane t of a quad takes c-th.
-template <int HD>
+// The 16-byte chunk of a K row that lane t of a quad takes c-th: neighbours under the boxes' swizzle, four lanes' whole
+// sectors in a lane's own copies.
+template <int HD, bool WHOLE>
 __device__ __forceinline__ int k_chunk(int t, int c) {
-  return HD == 64 ? t : (c >> 1) * 8 + 2 * t + (c & 1);
+  return HD == 64 ? t : WHOLE ? (c >> 1) * 8 + 2 * t + (c & 1) : 4 * c + t;
 }
 
 template <typename T, int HD, int NT, bool WHOLE>
@@ -429,7 +420,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
         const uint8_t* src = o >= 0 ? static_cast<const uint8_t*>(p.kv.k) + o : none;
 #pragma unroll
         for (int c = 0; c < G::KC; ++c)
-          copy_async<16>(smem_u32(buf) + ((i * G::KC + c) * 32 + lane) * 16, src + k_chunk<HD>(tl, c) * 16, o >= 0);
+          copy_async<16>(smem_u32(buf) + ((i * G::KC + c) * 32 + lane) * 16, src + k_chunk<HD, WHOLE>(tl, c) * 16, o >= 0);
       }
     }
   };
@@ -489,20 +480,21 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
     const bool real = 8 * n + gl < heads;
     const T* q = static_cast<const T*>(p.q) + r * p.ldq +
                  static_cast<int64_t>(kvh * p.rep + h0 + (real ? 8 * n + gl : 0)) * HD;
-    float x[G::KC * 16];
-    uint32_t top = 0;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int WORDS = F32 ? 16 : 8;   // of 16 values
+    uint32_t x[G::KC * WORDS], top = 0;
 #pragma unroll
-    for (int c = 0; c < G::KC; ++c) load16(q + k_chunk<HD>(tl, c) * 16, p.q_vec, x + c * 16);
+    for (int c = 0; c < G::KC; ++c) load16(q + k_chunk<HD, WHOLE>(tl, c) * 16, p.q_vec, x + c * WORDS);
 #pragma unroll
-    for (int i = 0; i < G::KC * 16; ++i) {
-      x[i] = real ? x[i] : 0.f;
-      top = max(top, abs_bits(x[i]));
-    }
+    for (int i = 0; i < G::KC * WORDS; ++i)
+      top = F32 ? max(top, x[i] & 0x7fffffffu) : __vmaxu2(top, x[i] & 0x7fff7fffu);
+    if constexpr (!F32) top = max(top & 0xffff0000u, top << 16);
+    if (!real) top = 0;
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // 2^-e of the largest value as two factors, each inside fp32's range
     const int e = top < 0x00800000u ? (top ? -126 : 0) : static_cast<int>(top >> 23) - 127, e0 = e >> 1, e1 = e - e0;
-    const float f0 = __int_as_float((127 - e0) << 23), f1 = __int_as_float((127 - e1) << 23);
+    const float f0 = real ? __int_as_float((127 - e0) << 23) : 0.f, f1 = __int_as_float((127 - e1) << 23);
     const float back = p.scale_log2 * __int_as_float((127 + e0) << 23) * __int_as_float((127 + e1) << 23);
     fs[n][0] = __shfl_sync(0xffffffffu, back, 8 * tl);        // lane (2 tl, 0)
     fs[n][1] = __shfl_sync(0xffffffffu, back, 8 * tl + 4);
@@ -511,7 +503,10 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
       if ((ks & (WARPS - 1)) != warp) continue;
       float y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = x[4 * ks + i] * f0 * f1;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = F32 ? x[4 * ks + i] : i & 1 ? x[2 * ks + i / 2] & 0xffff0000u : x[2 * ks + i / 2] << 16;
+        y[i] = __uint_as_float(w) * f0 * f1;
+      }
       const uint2 hi = make_uint2(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]));
       qf[(n * G::PARTS * G::KS + ks) * 32] = hi;
       if constexpr (G::PARTS == 2) {
@@ -525,15 +520,15 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
   }
   __syncthreads();
 
-  // This lane's columns are heads 8 n + 2 tl and + 1 of each N tile n. ms and mos are the maxima as exponents are taken
-  // against them (safe_max).
-  float m[NT][2], mo[NT][2], ms[NT][2], mos[NT][2], l[NT][2], acc[NT][G::KS][4];
+  // This lane's columns are heads 8 n + 2 tl and + 1 of each N tile n. Maxima start below every finite score instead of at
+  // -infinity, so that no difference to them is of two infinities.
+  float m[NT][2], mo[NT][2], l[NT][2], acc[NT][G::KS][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      m[n][c] = mo[n][c] = -INFINITY;
-      ms[n][c] = mos[n][c] = l[n][c] = 0.f;
+      m[n][c] = mo[n][c] = LOWEST;
+      l[n][c] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < G::KS; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
@@ -561,8 +556,8 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
         for (int q = 0; q < G::PARTS; ++q) a[n][q][0] = a[n][q][1] = a[n][q][2] = a[n][q][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < G::KC; ++c) {
-        const int a0_at = WHOLE ? G::box_at(t * TILE + gl, k_chunk<HD>(tl, c)) : ((2 * t * G::KC + c) * 32 + lane) * 16;
-        const int a1_at = WHOLE ? G::box_at(t * TILE + gl + 8, k_chunk<HD>(tl, c)) : a0_at + G::KC * 512;
+        const int a0_at = WHOLE ? G::box_at(t * TILE + gl, k_chunk<HD, WHOLE>(tl, c)) : ((2 * t * G::KC + c) * 32 + lane) * 16;
+        const int a1_at = WHOLE ? G::box_at(t * TILE + gl + 8, k_chunk<HD, WHOLE>(tl, c)) : a0_at + G::KC * 512;
         const uint4 u = *reinterpret_cast<const uint4*>(kbuf + a0_at);
         const uint4 w = *reinterpret_cast<const uint4*>(kbuf + a1_at);
         const uint32_t ku[4] = {u.x, u.y, u.z, u.w}, kw[4] = {w.x, w.y, w.z, w.w};
@@ -609,11 +604,18 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            s[t][n][2 * k + c] *= fs[n][c] * ks;
-            if (left < STEP && key >= left) s[t][n][2 * k + c] = -INFINITY;
-          }
+          for (int c = 0; c < 2; ++c) s[t][n][2 * k + c] *= fs[n][c] * ks;
       }
+    if (left < STEP) {   // keys that are not visible
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (t * TILE + 8 * (c >> 1) + gl >= left) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[t][n][c] = -INFINITY;
+          }
+    }
     bool raise = false;
     float tm[NT][2], tmo[NT][2];
 #pragma unroll
@@ -638,10 +640,8 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
           }
           x = fmaxf(x, m[n][c]);
           y = fmaxf(y, mo[n][c]);
-          ms[n][c] = safe_max(x);
-          mos[n][c] = safe_max(y);
-          const float co = ex2(mo[n][c] - mos[n][c]);
-          l[n][c] *= ex2(m[n][c] - ms[n][c]);
+          const float co = ex2(mo[n][c] - y);
+          l[n][c] *= ex2(m[n][c] - x);
 #pragma unroll
           for (int i = 0; i < G::KS; ++i) {
             acc[n][i][c] *= co;
@@ -659,8 +659,8 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
         float w[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          l[n][c & 1] += ex2(s[t][n][c] - ms[n][c & 1]);
-          w[c] = ex2(s[t][n][c] + e[t][c >> 1] - mos[n][c & 1]);
+          l[n][c & 1] += ex2(s[t][n][c] - m[n][c & 1]);
+          w[c] = ex2(s[t][n][c] + e[t][c >> 1] - mo[n][c & 1]);
           if constexpr (G::PARTS == 2) w[c] *= mant[t][c >> 1];
         }
         const uint32_t p0 = pack_half2(w[0], w[1]), p1 = pack_half2(w[2], w[3]);
@@ -676,6 +676,14 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
     if (!wait(vbar, j)) {
       late = 2;
       break;
+    }
+    if (WHOLE && left < STEP) {   // whatever lies behind the last visible key, NaN codes too, becomes zeros
+      for (int i = lane; i < (STEP - left) * (HD / 16); i += 32) {
+        const int row = left + i / (HD / 16);
+        *reinterpret_cast<uint4*>(buf + (G::STAGES + j % G::STAGES) * G::STEP_BYTES + G::box_at(row, i % (HD / 16))) =
+            make_uint4(0, 0, 0, 0);
+      }
+      __syncwarp();
     }
     // V: words of four dims of this lane's four keys, paired by key.
 #pragma unroll
@@ -695,10 +703,6 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
           } else {
             const uint2 u = *reinterpret_cast<const uint2*>(src);
             v[i][0] = u.x, v[i][1] = u.y;
-          }
-          if (WHOLE && left < STEP && row >= left) {   // whatever lies behind the last visible key, NaN codes too
-#pragma unroll
-            for (int w = 0; w < G::VB / 4; ++w) v[i][w] = 0;
           }
         }
 #pragma unroll
@@ -747,7 +751,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int h = warp * 8 * NT + 8 * n + 2 * tl + c;
-      const float f = exp2f(mos[n][c] - ms[n][c]);
+      const float f = exp2f(mo[n][c] - m[n][c]);
 #pragma unroll
       for (int i = 0; i < G::KS; ++i)
         *reinterpret_cast<float2*>(osm + h * G::O_ROW + i / (G::VB / 2) * 128 + gl * G::VB + 2 * (i % (G::VB / 2))) =
@@ -760,12 +764,12 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
   __syncthreads();
   const int64_t part0 = (r * p.nh + kvh * p.rep + h0) * p.splits + split;   // head h: part0 + h * splits
   for (int h = threadIdx.x; h < heads; h += blockDim.x) {
-    float top = -INFINITY, total = 0.f, f[WARPS];
+    float top = LOWEST, total = 0.f, f[WARPS];
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) top = fmaxf(top, msm[2 * (w * 8 * NT + h)]);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      f[w] = ex2(msm[2 * (w * 8 * NT + h)] - safe_max(top));
+      f[w] = ex2(msm[2 * (w * 8 * NT + h)] - top);
       total += f[w] * msm[2 * (w * 8 * NT + h) + 1];
     }
 #pragma unroll
@@ -858,62 +862,94 @@ int launch_t(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
 
 }  // namespace tc
 
-// Joins the splits of a (row, head): weights exp2(m_split - m) to shared memory, then the threads take two dims each of
-// every GROUPS-th split, GROUPS = 128 / (hd / 2, rounded up to a power of two).
+// Joins the splits of a (row, head), W warps (1 or 4) each: weights exp2(m_split - m), then four interleaved sums over the
+// splits, joined pairwise; the order, and so the bits, are the same for both W. One warp each where there are many
+// (row, head) pairs (64 rows x 32 heads of 9 splits: 2 us less than a CTA each), four where there are few and a
+// warp's loads would come one after another (1 row x 32 heads of 8 splits: 1.4 us less).
 constexpr int MAX_SPLITS = ONE_WAVE;
-template <typename T>
+template <typename T, int W>
 __global__ void __launch_bounds__(128) quant_combine_kernel(Params p) {
   pdl_trigger();
   pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
-  __shared__ float w[MAX_SPLITS], red[8];
-  __shared__ float2 sums[128];
-  const int64_t r = blockIdx.y;
-  const int h = blockIdx.x, hd = p.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t n_vis = visible(p, r), base = (r * p.nh + h) * p.splits, per = split_keys(n_vis, p.nkv);
+  constexpr int TEAMS = 4 / W;
+  __shared__ float weights[TEAMS][MAX_SPLITS];
+  __shared__ float2 sums[4][64];   // W = 4: the warps' sums of 64 columns (pairs of dims)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = p.hd, cols = hd / 2, team = warp / W;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * TEAMS + team;
+  if (id >= static_cast<int64_t>(p.B) * p.nh) return;   // W = 1: whole warps, which no barrier joins
+  const int64_t r = id / p.nh, base = id * p.splits;
+  const int64_t n_vis = visible(p, r), per = split_keys(n_vis, p.nkv);
   const int used = static_cast<int>((n_vis + per - 1) / per);
-  const float2* ml = reinterpret_cast<const float2*>(p.ws + static_cast<int64_t>(gridDim.y) * p.nh * p.splits * hd) + base;
-  float top = -INFINITY;
-  for (int s = tid; s < used; s += 128) {
-    w[s] = ml[s].x;
-    top = fmaxf(top, w[s]);
-  }
+  const float2* ml = reinterpret_cast<const float2*>(p.ws + static_cast<int64_t>(p.B) * p.nh * p.splits * hd) + base;
+  const float2* src = reinterpret_cast<const float2*>(p.ws + base * hd);
+  T* dst = static_cast<T*>(p.out) + r * p.ldo + (id - r * p.nh) * hd;
+  float* w = weights[team];
+  float top = -INFINITY, total = 0.f;
+  for (int s = lane; s < used; s += 32) top = fmaxf(top, ml[s].x);
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-  if (lane == 0) red[warp] = top;
-  __syncthreads();
-  top = safe_max(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-  float total = 0.f;
-  for (int s = tid; s < used; s += 128) {
-    w[s] = exp2f(w[s] - top);
-    total += w[s] * ml[s].y;
+  top = safe_max(top);
+  for (int s = lane; s < used; s += 32) {
+    const float2 v = ml[s];
+    const float f = exp2f(v.x - top);
+    total = fmaf(f, v.y, total);
+    if (W == 1 || warp == 0) w[s] = f;
   }
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
-  if (lane == 0) red[4 + warp] = total;
-  __syncthreads();
-  total = red[4] + red[5] + red[6] + red[7];
-  const int cols = hd / 2, width = cols <= 1 ? 1 : 1 << (32 - __clz(cols - 1)), groups = 128 / width;
-  const int col = tid & (width - 1), group = tid / width;
-  float2 o = make_float2(0.f, 0.f);
-  if (col < cols) {
-    const float2* src = reinterpret_cast<const float2*>(p.ws + base * hd) + col;
-#pragma unroll 8
-    for (int s = group; s < used; s += groups) {
-      const float2 x = src[static_cast<int64_t>(s) * cols];
-      o.x = fmaf(w[s], x.x, o.x);
-      o.y = fmaf(w[s], x.y, o.y);
+  if constexpr (W == 1) __syncwarp(); else __syncthreads();
+  for (int c0 = 0; c0 < cols; c0 += 64) {   // two columns a lane at a time
+    const int c = c0 + lane, d = c + 32;
+    constexpr int SUMS = W == 1 ? 4 : 1;
+    float2 a[SUMS], b[SUMS];
+#pragma unroll
+    for (int g = 0; g < SUMS; ++g) a[g] = b[g] = make_float2(0.f, 0.f);
+#pragma unroll(W == 1 ? 2 : 8)
+    for (int s0 = W == 1 ? 0 : warp; s0 < used; s0 += 4) {
+#pragma unroll
+      for (int g = 0; g < SUMS; ++g) {
+        const int s = s0 + g;
+        if (s < used) {
+          const float f = w[s];
+          if (c < cols) {
+            const float2 x = src[static_cast<int64_t>(s) * cols + c];
+            a[g].x = fmaf(f, x.x, a[g].x);
+            a[g].y = fmaf(f, x.y, a[g].y);
+          }
+          if (d < cols) {
+            const float2 y = src[static_cast<int64_t>(s) * cols + d];
+            b[g].x = fmaf(f, y.x, b[g].x);
+            b[g].y = fmaf(f, y.y, b[g].y);
+          }
+        }
+      }
     }
-  }
-  sums[tid] = o;
-  __syncthreads();
-  if (tid < cols) {
-    for (int g = 1; g < groups; ++g) {
-      o.x += sums[g * width + tid].x;
-      o.y += sums[g * width + tid].y;
+    if constexpr (W == 1) {
+      a[0].x = (a[0].x + a[1].x) + (a[2].x + a[3].x);
+      a[0].y = (a[0].y + a[1].y) + (a[2].y + a[3].y);
+      b[0].x = (b[0].x + b[1].x) + (b[2].x + b[3].x);
+      b[0].y = (b[0].y + b[1].y) + (b[2].y + b[3].y);
+    } else {
+      __syncthreads();   // the columns before these are read
+      sums[warp][lane] = a[0];
+      sums[warp][lane + 32] = b[0];
+      __syncthreads();
+      if (warp == 0) {
+        a[0].x = (sums[0][lane].x + sums[1][lane].x) + (sums[2][lane].x + sums[3][lane].x);
+        a[0].y = (sums[0][lane].y + sums[1][lane].y) + (sums[2][lane].y + sums[3][lane].y);
+      } else if (warp == 1) {
+        b[0].x = (sums[0][lane + 32].x + sums[1][lane + 32].x) + (sums[2][lane + 32].x + sums[3][lane + 32].x);
+        b[0].y = (sums[0][lane + 32].y + sums[1][lane + 32].y) + (sums[2][lane + 32].y + sums[3][lane + 32].y);
+      }
     }
-    T* dst = static_cast<T*>(p.out) + r * p.ldo + static_cast<int64_t>(h) * hd + 2 * tid;
-    dst[0] = from_f<T>(n_vis == 0 ? 0.f : o.x / total);
-    dst[1] = from_f<T>(n_vis == 0 ? 0.f : o.y / total);
+    if ((W == 1 || warp == 0) && c < cols) {
+      dst[2 * c] = from_f<T>(n_vis == 0 ? 0.f : a[0].x / total);
+      dst[2 * c + 1] = from_f<T>(n_vis == 0 ? 0.f : a[0].y / total);
+    }
+    if ((W == 1 || warp == 1) && d < cols) {
+      dst[2 * d] = from_f<T>(n_vis == 0 ? 0.f : b[0].x / total);
+      dst[2 * d + 1] = from_f<T>(n_vis == 0 ? 0.f : b[0].y / total);
+    }
   }
 }
 
@@ -938,7 +974,11 @@ template <typename T>
 int launch_t(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
   if (tc::supported(p) ? tc::launch_t<T>(p, B, nkv, st) : launch_any<T>(p, B, nkv, st)) return -1;
   if (p.splits == 1) return 0;
-  launch_pdl_async(quant_combine_kernel<T>, dim3(static_cast<unsigned>(p.nh), static_cast<unsigned>(B)), 128, 0, st, p);
+  const int64_t pairs = B * p.nh;
+  if (pairs >= 1024)
+    launch_pdl_async(quant_combine_kernel<T, 1>, static_cast<unsigned>((pairs + 3) / 4), 128, 0, st, p);
+  else
+    launch_pdl_async(quant_combine_kernel<T, 4>, static_cast<unsigned>(pairs), 128, 0, st, p);
   return check_launch("quant_combine_kernel");
 }
 
@@ -967,6 +1007,7 @@ int launch(int dtype, const void* q, int64_t ldq, const KVCache& kv, const KVSca
   p.positions = positions;
   p.out = out;
   p.ldo = ldo;
+  p.B = static_cast<int>(B);
   p.nh = static_cast<int>(nh);
   p.rep = static_cast<int>(nh / nkv);
   p.hd = static_cast<int>(hd);

@@ -480,6 +480,25 @@ def test_decode_is_independent_of_batch_and_table_width():
         assert torch.equal(one[0], whole[r])
 
 
+@pytest.mark.parametrize("dtype,nh,nkv,hd,bs", [(torch.bfloat16, 32, 4, 128, 16), (torch.float32, 32, 16, 64, 16),
+                                                (torch.bfloat16, 32, 8, 128, 20), (torch.bfloat16, 32, 8, 80, 16)])
+def test_decode_bits_do_not_depend_on_the_batch(dtype, nh, nkv, hd, bs):
+    """Rows of a batch large enough for another join, and behind a table of other width, against each row alone."""
+    lengths = [1 + (i * 797) % 3000 for i in range(40)]
+    q, pools, table, positions, n_slots = decode_case(dtype, lengths, nh, nkv, hd, bs, seed=11)
+    whole = torch.empty_like(q)
+    ops.attention_decode_quant(q, ops.quant_paged_desc(*pools, table), n_slots, positions, whole, 40, nh, nkv, hd)
+    wide = torch.cat([table] * 14, 1)
+    out = torch.empty_like(q)
+    ops.attention_decode_quant(q, ops.quant_paged_desc(*pools, wide), 14 * n_slots, positions, out, 40, nh, nkv, hd)
+    assert torch.equal(out, whole)
+    for r in (0, 7, 19, 39):
+        one = torch.empty_like(q[:1])
+        ops.attention_decode_quant(q[r: r + 1], ops.quant_paged_desc(*pools, table[r: r + 1]), n_slots,
+                                   positions[r: r + 1], one, 1, nh, nkv, hd)
+        assert torch.equal(one[0], whole[r])
+
+
 def test_pool_slices_and_strided_rows():
     """Heads of a larger pool, rows of q and out inside wider tensors, a table cut from a wider one."""
     nkv, hd, bs, nh = 2, 128, 16, 8
