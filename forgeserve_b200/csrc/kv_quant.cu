@@ -20,6 +20,12 @@
 
 namespace fs {
 
+#ifndef WHEADS
+#define WHEADS 2
+#endif
+#ifndef RU
+#define RU 2
+#endif
 namespace {
 
 struct WriteParams {
@@ -146,6 +152,203 @@ __global__ void __launch_bounds__(256) rotary_write_kernel(WriteParams p, int in
   }
 }
 
+// A 16-byte piece as fp32, and back with one rounding.
+__device__ __forceinline__ void load_piece(const __nv_bfloat16* p, float* x) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load_piece(const float* p, float* x) {
+  *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void store_piece(__nv_bfloat16* p, const float* x) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+}
+__device__ __forceinline__ void store_piece(float* p, const float* x) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+// N (2, 4 or 8) table values, N-aligned.
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float* x) {
+  if constexpr (N == 2) {
+    *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(p + i);
+  }
+}
+// N (4 or 8) codes, and their values.
+template <int N>
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p) {
+  if constexpr (N == 8) return *reinterpret_cast<const uint2*>(p);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(p), 0);
+}
+template <int N>
+__device__ __forceinline__ void decode_piece(uint2 codes, float scale, float* x) {
+  const uint32_t w[2] = {codes.x, codes.y};
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const uint32_t h = e4m3x2_to_half2(static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1))));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    x[2 * i] = f.x * scale;
+    x[2 * i + 1] = f.y * scale;
+  }
+}
+// The codes of N (4 or 8) values.
+template <int N>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float* x, float inv) {
+  uint32_t w[N / 4];
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i)
+    w[i] = e4m3x2(x[4 * i] * inv, x[4 * i + 1] * inv) | e4m3x2(x[4 * i + 2] * inv, x[4 * i + 3] * inv) << 16;
+  if constexpr (N == 8)
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else
+    *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+
+// The vector form, for heads of whole 16-byte pieces (write_vec_ok). A thread owns two pieces of VEC values of a head,
+// chosen so that the lanes of a head read neighbouring pieces: x[VEC c ..] and x[r/2 + VEC c ..] where they turn as pairs
+// (half layout), the same distance apart in the copied rest; first and second half of the head otherwise. It does so for
+// HEADS heads of its token, so that its cos and sin are read once and its loads are in flight together. The lanes of a
+// head (a power of two, some idle where hd / (2 VEC) is none) find the largest |x| by shuffles.
+template <typename T, bool QUANT, bool IL>
+__global__ void __launch_bounds__(256) rotary_write_vec_kernel(WriteParams p, int lanes, unsigned groups) {
+  pdl_trigger();
+  pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T)), HEADS = WHEADS;
+  const unsigned item = (blockIdx.x * 256u + threadIdx.x) / lanes;
+  const int c = threadIdx.x & (lanes - 1);
+  const unsigned tok = item / groups, hg = item - tok * groups;
+  const int heads = p.nh + 2 * p.nkv, half = p.rd / 2;
+  const bool in = tok < p.tokens && c * 2 * VEC < p.hd;
+  const T* row = static_cast<const T*>(p.qkv) + tok * p.ld;
+
+  // Where the pieces of q and k heads lie, and of v heads.
+  const bool turns = IL || c * 2 * VEC < p.rd;   // IL: pair by pair below
+  int lo = VEC * c, hi = p.hd / 2 + VEC * c;
+  const int lo_v = lo, hi_v = hi;
+  if (!IL) {
+    if (turns) {
+      hi = half + VEC * c;
+    } else {
+      lo = p.rd + VEC * c - half;   // c - rd / (2 VEC) pieces into the rest
+      hi = lo + (p.hd - p.rd) / 2;
+    }
+  }
+  float x[HEADS][2 * VEC];
+#pragma unroll
+  for (int u = 0; u < HEADS; ++u) {
+    const int h = hg + u * groups;
+    if (in && h < heads) {
+      const bool v = h >= p.nh + p.nkv;
+      load_piece(row + h * p.hd + (v ? lo_v : lo), x[u]);
+      load_piece(row + h * p.hd + (v ? hi_v : hi), x[u] + VEC);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * VEC; ++i) x[u][i] = 0.f;
+    }
+  }
+  const int64_t pos = in ? p.positions[tok] : -1;
+  const bool report = c == 0 && hg == 0;
+  const bool ok = in && token_ok(p, pos, report);
+  Slot at = {-1, -1};
+  if (ok) at = find_slot(p, tok, pos, report);
+  // cos and sin of the thread's VEC pairs. Pairs past the rotated ones are left alone (not turned by 1 and 0: a NaN or an
+  // infinity stays in its own value).
+  float cs[VEC], sn[VEC];
+  auto pair_of = [&](int i) { return IL ? (i < VEC / 2 ? lo / 2 + i : hi / 2 + i - VEC / 2) : VEC * c + i; };
+  if (ok && hg < static_cast<unsigned>(p.nh + p.nkv)) {
+    const float* ct = p.cos_t + pos * half;
+    const float* st = p.sin_t + pos * half;
+    if (!IL) {
+      if (turns) {
+        load_floats<VEC>(ct + VEC * c, cs);
+        load_floats<VEC>(st + VEC * c, sn);
+      }
+    } else if (half % (VEC / 2) == 0) {
+#pragma unroll
+      for (int i = 0; i < VEC; i += VEC / 2) {
+        if (pair_of(i) < half) {
+          load_floats<VEC / 2>(ct + pair_of(i), cs + i);
+          load_floats<VEC / 2>(st + pair_of(i), sn + i);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (pair_of(i) < half) cs[i] = ct[pair_of(i)], sn[i] = st[pair_of(i)];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < HEADS; ++u) {
+    const int h = hg + u * groups;
+    const bool v = h >= p.nh + p.nkv;
+    if (ok && !v) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if (pair_of(i) < half) {
+          float& a = x[u][IL ? 2 * i : i];
+          float& b = x[u][IL ? 2 * i + 1 : VEC + i];
+          const float a0 = a, b0 = b;
+          a = a0 * cs[i] - b0 * sn[i];
+          b = b0 * cs[i] + a0 * sn[i];
+        }
+      }
+    }
+    if (ok && h < p.nh) {
+      T* o = static_cast<T*>(p.q_out) + tok * p.ldq + h * p.hd;
+      store_piece(o + lo, x[u]);
+      store_piece(o + hi, x[u] + VEC);
+    }
+    const int g = h - p.nh - (v ? p.nkv : 0);
+    const bool put = h >= p.nh && h < heads && at.values >= 0;
+    const int l0 = v ? lo_v : lo, l1 = v ? hi_v : hi;
+    if constexpr (QUANT) {
+      if (!__any_sync(0xffffffffu, put)) continue;   // a warp of q heads
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 2 * VEC; ++i) top = max(top, abs_bits(x[u][i]));
+      for (int o = lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (put) {
+        const float scale = row_scale(top), inv = 1.f / scale;
+        uint8_t* o = static_cast<uint8_t*>(v ? p.kv.v : p.kv.k) + at.values + g * p.kv.head_stride;
+        store_codes<VEC>(o + l0, x[u], inv);
+        store_codes<VEC>(o + l1, x[u] + VEC, inv);
+        if (c == 0) (v ? p.sc.v : p.sc.k)[at.scale + g * p.sc.head_stride] = scale;
+      }
+    } else if (put) {
+      T* o = static_cast<T*>(v ? p.kv.v : p.kv.k) + at.values + g * p.kv.head_stride;
+      store_piece(o + l0, x[u]);
+      store_piece(o + l1, x[u] + VEC);
+    }
+  }
+}
+
+// Whole 16-byte pieces everywhere: heads of 2 VEC values' multiples (the rotated part too, in the half layout), rows,
+// tables and cache on their boundaries.
+template <typename T>
+bool write_vec_ok(const WriteParams& p, bool quant, bool il) {
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+  if (p.hd % (2 * VEC) || p.hd > 64 * VEC || (!il && p.rd % (2 * VEC))) return false;
+  const int64_t el = quant ? 16 : VEC;   // elements of the cache in 16 bytes
+  if (p.ld % VEC || (p.nh > 0 && p.ldq % VEC) || p.kv.block_stride % el || p.kv.head_stride % el) return false;
+  if (quant && p.hd % 16) return false;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(p.qkv) | (p.nh > 0 ? reinterpret_cast<uintptr_t>(p.q_out) : 0) |
+                        (p.rd > 0 ? reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t) : 0) |
+                        reinterpret_cast<uintptr_t>(p.kv.k) | reinterpret_cast<uintptr_t>(p.kv.v);
+  return (all & 15) == 0;
+}
+
 // Values of `n_slots` slots of every row, k and v: one thread a value of each.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -175,8 +378,68 @@ __global__ void __launch_bounds__(256)
   v_out[o] = from_f<T>(v);
 }
 
+// The vector form: heads of whole VEC-value pieces, 16 bytes of each output at a time. A thread keeps its place in the
+// rows and takes U slots, its loads of codes and scales in flight together.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    kv_dequant_vec_kernel(KVCache kv, KVScales sc, uint32_t n_slots, int nkv, int hd, T* __restrict__ k_out,
+                          T* __restrict__ v_out, unsigned* err) {
+  pdl_trigger();
+  pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T)), U = RU;
+  const int lanes = hd / VEC, rows = 256 / lanes, c = threadIdx.x % lanes, i0 = threadIdx.x / lanes;
+  const int64_t r = blockIdx.z, g = blockIdx.y;
+  if (i0 >= rows) return;
+  const uint32_t s0 = blockIdx.x * (rows * U) + i0;
+  uint2 ck[U], cv[U];
+  float sk[U], sv[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t s = s0 + u * rows;
+    ck[u] = cv[u] = make_uint2(0, 0);
+    sk[u] = sv[u] = 0.f;
+    if (s < n_slots) {
+      int64_t col, in;
+      split_slot(s, kv.block_size, col, in);
+      const int64_t blk = col < kv.table_cols ? kv.table[r * kv.table_stride + col] : -1;
+      if (blk >= 0 && blk < kv.num_blocks) {
+        const int64_t at = blk * kv.block_stride + g * kv.head_stride + in * hd + c * VEC;
+        const int64_t sat = blk * sc.block_stride + g * sc.head_stride + in;
+        ck[u] = load_codes<VEC>(static_cast<const uint8_t*>(kv.k) + at);
+        cv[u] = load_codes<VEC>(static_cast<const uint8_t*>(kv.v) + at);
+        sk[u] = sc.k[sat];
+        sv[u] = sc.v[sat];
+      } else if (c == 0 && in == 0) {
+        flag_error(err, ERR_BAD_SLOT);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t s = s0 + u * rows;
+    if (s >= n_slots) break;
+    const int64_t o = ((r * nkv + g) * n_slots + s) * hd + c * VEC;
+    float x[VEC];
+    decode_piece<VEC>(ck[u], sk[u], x);
+    store_piece(k_out + o, x);
+    decode_piece<VEC>(cv[u], sv[u], x);
+    store_piece(v_out + o, x);
+  }
+}
+
 template <typename T>
 int write_t(const WriteParams& p, bool quant, int interleaved, cudaStream_t st) {
+  constexpr int PIECES = 32 / static_cast<int>(sizeof(T));   // values a lane of the vector form holds of a head
+  int lanes = 1;
+  while (lanes * PIECES < p.hd) lanes *= 2;
+  const unsigned groups = (p.nh + 2 * p.nkv + WHEADS - 1) / WHEADS;
+  const int64_t vec_blocks = (p.tokens * groups * lanes + 255) / 256;
+  if (write_vec_ok<T>(p, quant, interleaved) && vec_blocks < (1 << 24)) {   // thread numbers of 32 bits
+    auto kernel = quant ? (interleaved ? rotary_write_vec_kernel<T, true, true> : rotary_write_vec_kernel<T, true, false>)
+                        : (interleaved ? rotary_write_vec_kernel<T, false, true> : rotary_write_vec_kernel<T, false, false>);
+    launch_pdl_async(kernel, static_cast<unsigned>(vec_blocks), 256, 0, st, p, lanes, groups);
+    return check_launch("rotary_write_vec_kernel");
+  }
   const int64_t warps = p.tokens * (p.nh + 2 * p.nkv), blocks = (warps + 7) / 8;
   if (blocks > INT32_MAX) return fail("rotary_kv_write: too many tokens");
   if (quant)
@@ -221,16 +484,23 @@ int kv_dequant(int dtype, const KVCache& kv, const KVScales& sc, int64_t B, int6
                void* k_out, void* v_out, cudaStream_t st) {
   unsigned* err = error_word();
   if (!err) return -1;
-  const dim3 grid(static_cast<unsigned>((n_slots * hd + 255) / 256), static_cast<unsigned>(nkv),
-                  static_cast<unsigned>(B));
+  const int vec = dtype == F32 ? 4 : 8;
+  const uintptr_t out = reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out);
+  const uintptr_t in = reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v);
+  const bool pieces = hd % vec == 0 && hd <= 256 * vec && (out & 15) == 0 && (in & (vec - 1)) == 0 &&
+                      kv.block_stride % vec == 0 && kv.head_stride % vec == 0;
+  const int64_t a_block = pieces ? 256 / (hd / vec) * RU : 0;   // slots
+  const int64_t blocks = pieces ? (n_slots + a_block - 1) / a_block : (n_slots * hd + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(nkv), static_cast<unsigned>(B));
+  auto run = [&](auto* k, auto* v) {
+    using T = std::remove_pointer_t<decltype(k)>;
+    launch_pdl_async(pieces ? kv_dequant_vec_kernel<T> : kv_dequant_kernel<T>, grid, 256, 0, st, kv, sc,
+                     static_cast<uint32_t>(n_slots), static_cast<int>(nkv), static_cast<int>(hd), k, v, err);
+  };
   if (dtype == F32)
-    launch_pdl_async(kv_dequant_kernel<float>, grid, 256, 0, st, kv, sc, static_cast<uint32_t>(n_slots),
-                     static_cast<int>(nkv), static_cast<int>(hd), static_cast<float*>(k_out),
-                     static_cast<float*>(v_out), err);
+    run(static_cast<float*>(k_out), static_cast<float*>(v_out));
   else
-    launch_pdl_async(kv_dequant_kernel<__nv_bfloat16>, grid, 256, 0, st, kv, sc, static_cast<uint32_t>(n_slots),
-                     static_cast<int>(nkv), static_cast<int>(hd), static_cast<__nv_bfloat16*>(k_out),
-                     static_cast<__nv_bfloat16*>(v_out), err);
+    run(static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out));
   return check_launch("kv_dequant_kernel");
 }
 
