@@ -20,12 +20,6 @@
 
 namespace fs {
 
-#ifndef WHEADS
-#define WHEADS 2
-#endif
-#ifndef RU
-#define RU 2
-#endif
 namespace {
 
 struct WriteParams {
@@ -52,12 +46,12 @@ struct Slot {
   int64_t values, scale;
 };
 __device__ __forceinline__ Slot find_slot(const WriteParams& p, int64_t tok, int64_t pos, bool report) {
-  const int64_t r = tok / p.T_new;
-  const int64_t slot = p.slot_from_pos ? pos : p.slot_base + (tok - r * p.T_new);
+  const uint32_t r = static_cast<uint32_t>(tok) / static_cast<uint32_t>(p.T_new);   // tokens are below 2^31
+  const int64_t slot = p.slot_from_pos ? pos : p.slot_base + (tok - static_cast<int64_t>(r) * p.T_new);
   int64_t col, in;
   split_slot(slot, p.kv.block_size, col, in);
   int64_t blk = -1;
-  if (col < p.kv.table_cols) blk = p.kv.table[r * p.kv.table_stride + col];
+  if (col < p.kv.table_cols) blk = p.kv.table[static_cast<int64_t>(r) * p.kv.table_stride + col];
   if (blk < 0 || blk >= p.kv.num_blocks) {
     if (report) flag_error(p.err, ERR_BAD_SLOT);
     return {-1, -1};
@@ -131,7 +125,7 @@ __global__ void __launch_bounds__(256) rotary_write_kernel(WriteParams p, int in
   if constexpr (QUANT) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float scale = row_scale(top), inv = 1.f / scale;
+    const float scale = row_scale(top), inv = inverse(scale);
     uint8_t* o = static_cast<uint8_t*>(is_v ? p.kv.v : p.kv.k) + at.values + static_cast<int64_t>(g) * p.kv.head_stride;
 #pragma unroll
     for (int j = 0; j < MAXP; ++j) {
@@ -152,9 +146,8 @@ __global__ void __launch_bounds__(256) rotary_write_kernel(WriteParams p, int in
   }
 }
 
-// A 16-byte piece as fp32, and back with one rounding.
-__device__ __forceinline__ void load_piece(const __nv_bfloat16* p, float* x) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
+// A 16-byte piece as fp32 values, and back with one rounding.
+__device__ __forceinline__ void unpack_piece(uint4 u, float* x, const __nv_bfloat16*) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -162,8 +155,10 @@ __device__ __forceinline__ void load_piece(const __nv_bfloat16* p, float* x) {
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
-__device__ __forceinline__ void load_piece(const float* p, float* x) {
-  *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+__device__ __forceinline__ void unpack_piece(uint4 u, float* x, const float*) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -216,23 +211,18 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float* x, float in
     *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 
-// The vector form, for heads of whole 16-byte pieces (write_vec_ok). A thread owns two pieces of VEC values of a head,
-// chosen so that the lanes of a head read neighbouring pieces: x[VEC c ..] and x[r/2 + VEC c ..] where they turn as pairs
-// (half layout), the same distance apart in the copied rest; first and second half of the head otherwise. It does so for
-// HEADS heads of its token, so that its cos and sin are read once and its loads are in flight together. The lanes of a
-// head (a power of two, some idle where hd / (2 VEC) is none) find the largest |x| by shuffles.
-template <typename T, bool QUANT, bool IL>
-__global__ void __launch_bounds__(256) rotary_write_vec_kernel(WriteParams p, int lanes, unsigned groups) {
+// The vector form, for heads of whole 16-byte pieces (write_vec_ok). A thread owns two pieces of VEC values
+// of a head, chosen so that the lanes of a head read neighbouring pieces: x[VEC c ..] and x[r/2 + VEC c ..] where they turn
+// as pairs (half layout), the same in the copied rest; first and second half of the head otherwise. It does so for HEADS
+// neighbouring heads, so that its cos and sin are read once and its loads are in flight together. The lanes of a head (a power of two,
+// some idle where hd / (2 VEC) is none) find the largest |x| by shuffles.
+template <typename T, bool QUANT, bool IL, int HEADS>
+__global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p, int lanes, unsigned groups) {
   pdl_trigger();
   pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
-  constexpr int VEC = 16 / static_cast<int>(sizeof(T)), HEADS = WHEADS;
-  const unsigned item = (blockIdx.x * 256u + threadIdx.x) / lanes;
-  const int c = threadIdx.x & (lanes - 1);
-  const unsigned tok = item / groups, hg = item - tok * groups;
-  const int heads = p.nh + 2 * p.nkv, half = p.rd / 2;
-  const bool in = tok < p.tokens && c * 2 * VEC < p.hd;
-  const T* row = static_cast<const T*>(p.qkv) + tok * p.ld;
-
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+  const int c = threadIdx.x & (lanes - 1), heads = p.nh + 2 * p.nkv, half = p.rd / 2;
+  const unsigned per = 256u / lanes, items = static_cast<unsigned>(p.tokens) * groups;
   // Where the pieces of q and k heads lie, and of v heads.
   const bool turns = IL || c * 2 * VEC < p.rd;   // IL: pair by pair below
   int lo = VEC * c, hi = p.hd / 2 + VEC * c;
@@ -245,37 +235,33 @@ __global__ void __launch_bounds__(256) rotary_write_vec_kernel(WriteParams p, in
       hi = lo + (p.hd - p.rd) / 2;
     }
   }
-  float x[HEADS][2 * VEC];
-#pragma unroll
-  for (int u = 0; u < HEADS; ++u) {
-    const int h = hg + u * groups;
-    if (in && h < heads) {
-      const bool v = h >= p.nh + p.nkv;
-      load_piece(row + h * p.hd + (v ? lo_v : lo), x[u]);
-      load_piece(row + h * p.hd + (v ? hi_v : hi), x[u] + VEC);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2 * VEC; ++i) x[u][i] = 0.f;
-    }
-  }
-  const int64_t pos = in ? p.positions[tok] : -1;
-  const bool report = c == 0 && hg == 0;
-  const bool ok = in && token_ok(p, pos, report);
-  Slot at = {-1, -1};
-  if (ok) at = find_slot(p, tok, pos, report);
-  // cos and sin of the thread's VEC pairs. Pairs past the rotated ones are left alone (not turned by 1 and 0: a NaN or an
-  // infinity stays in its own value).
-  float cs[VEC], sn[VEC];
-  auto pair_of = [&](int i) { return IL ? (i < VEC / 2 ? lo / 2 + i : hi / 2 + i - VEC / 2) : VEC * c + i; };
-  if (ok && hg < static_cast<unsigned>(p.nh + p.nkv)) {
+  // Items are (token, HEADS heads). All lanes of a warp stay until its last item is done.
+  const unsigned step = gridDim.x * per;
+  unsigned item = blockIdx.x * per + threadIdx.x / lanes;
+  int64_t next_pos = item < items ? p.positions[item / groups] : -1;
+  while (__any_sync(0xffffffffu, item < items)) {
+    const unsigned token = item / groups;
+    const int h0 = (item - token * groups) * HEADS;
+    const int64_t tok = token, pos = next_pos;
+    const bool ok = item < items && c * 2 * VEC < p.hd && token_ok(p, pos, c == 0 && h0 == 0);
+    const unsigned next = item + step;
+    next_pos = next < items ? p.positions[next / groups] : -1;
+    const T* row = static_cast<const T*>(p.qkv) + tok * p.ld;
+    T* q_row = static_cast<T*>(p.q_out) + tok * p.ldq;
+    Slot at = {-1, -1};
+    if (ok && h0 + HEADS > p.nh) at = find_slot(p, tok, pos, c == 0 && h0 <= p.nh);
+    // cos and sin of the thread's VEC pairs. Pairs past the rotated ones are left alone (not turned by 1 and 0: a NaN or an
+    // infinity stays in its own value).
+    float cs[VEC], sn[VEC];
+    auto pair_of = [&](int i) { return IL ? (i < VEC / 2 ? lo / 2 + i : hi / 2 + i - VEC / 2) : VEC * c + i; };
     const float* ct = p.cos_t + pos * half;
     const float* st = p.sin_t + pos * half;
     if (!IL) {
-      if (turns) {
+      if (ok && turns) {
         load_floats<VEC>(ct + VEC * c, cs);
         load_floats<VEC>(st + VEC * c, sn);
       }
-    } else if (half % (VEC / 2) == 0) {
+    } else if (ok && half % (VEC / 2) == 0) {
 #pragma unroll
       for (int i = 0; i < VEC; i += VEC / 2) {
         if (pair_of(i) < half) {
@@ -283,54 +269,68 @@ __global__ void __launch_bounds__(256) rotary_write_vec_kernel(WriteParams p, in
           load_floats<VEC / 2>(st + pair_of(i), sn + i);
         }
       }
-    } else {
+    } else if (ok) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
         if (pair_of(i) < half) cs[i] = ct[pair_of(i)], sn[i] = st[pair_of(i)];
     }
-  }
+    uint4 raw[HEADS][2];
 #pragma unroll
-  for (int u = 0; u < HEADS; ++u) {
-    const int h = hg + u * groups;
-    const bool v = h >= p.nh + p.nkv;
-    if (ok && !v) {
+    for (int u = 0; u < HEADS; ++u) {
+      const int h = h0 + u;
+      raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
+      if (ok && h < heads) {
+        const bool v = h >= p.nh + p.nkv;
+        raw[u][0] = *reinterpret_cast<const uint4*>(row + h * p.hd + (v ? lo_v : lo));
+        raw[u][1] = *reinterpret_cast<const uint4*>(row + h * p.hd + (v ? hi_v : hi));
+      }
+    }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (pair_of(i) < half) {
-          float& a = x[u][IL ? 2 * i : i];
-          float& b = x[u][IL ? 2 * i + 1 : VEC + i];
-          const float a0 = a, b0 = b;
-          a = a0 * cs[i] - b0 * sn[i];
-          b = b0 * cs[i] + a0 * sn[i];
+    for (int u = 0; u < HEADS; ++u) {
+      const int h = h0 + u;
+      const bool v = h >= p.nh + p.nkv, mine = ok && h < heads;
+      float x[2 * VEC];
+      unpack_piece(raw[u][0], x, static_cast<const T*>(nullptr));
+      unpack_piece(raw[u][1], x + VEC, static_cast<const T*>(nullptr));
+      if (!v) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          if (pair_of(i) < half) {
+            float& a = x[IL ? 2 * i : i];
+            float& b = x[IL ? 2 * i + 1 : VEC + i];
+            const float a0 = a, b0 = b;
+            a = a0 * cs[i] - b0 * sn[i];
+            b = b0 * cs[i] + a0 * sn[i];
+          }
         }
       }
-    }
-    if (ok && h < p.nh) {
-      T* o = static_cast<T*>(p.q_out) + tok * p.ldq + h * p.hd;
-      store_piece(o + lo, x[u]);
-      store_piece(o + hi, x[u] + VEC);
-    }
-    const int g = h - p.nh - (v ? p.nkv : 0);
-    const bool put = h >= p.nh && h < heads && at.values >= 0;
-    const int l0 = v ? lo_v : lo, l1 = v ? hi_v : hi;
-    if constexpr (QUANT) {
-      if (!__any_sync(0xffffffffu, put)) continue;   // a warp of q heads
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 2 * VEC; ++i) top = max(top, abs_bits(x[u][i]));
-      for (int o = lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (put) {
-        const float scale = row_scale(top), inv = 1.f / scale;
-        uint8_t* o = static_cast<uint8_t*>(v ? p.kv.v : p.kv.k) + at.values + g * p.kv.head_stride;
-        store_codes<VEC>(o + l0, x[u], inv);
-        store_codes<VEC>(o + l1, x[u] + VEC, inv);
-        if (c == 0) (v ? p.sc.v : p.sc.k)[at.scale + g * p.sc.head_stride] = scale;
+      if (mine && h < p.nh) {
+        store_piece(q_row + h * p.hd + lo, x);
+        store_piece(q_row + h * p.hd + hi, x + VEC);
       }
-    } else if (put) {
-      T* o = static_cast<T*>(v ? p.kv.v : p.kv.k) + at.values + g * p.kv.head_stride;
-      store_piece(o + l0, x[u]);
-      store_piece(o + l1, x[u] + VEC);
+      const int g = h - p.nh - (v ? p.nkv : 0);
+      const bool put = mine && h >= p.nh && at.values >= 0;
+      const int l0 = v ? lo_v : lo, l1 = v ? hi_v : hi;
+      if constexpr (QUANT) {
+        if (!__any_sync(0xffffffffu, put)) continue;   // a warp of q heads
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * VEC; ++i) top = max(top, abs_bits(x[i]));
+        for (int o = lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (put) {
+          const float scale = row_scale(top), inv = inverse(scale);
+          uint8_t* o = static_cast<uint8_t*>(v ? p.kv.v : p.kv.k) + at.values + g * p.kv.head_stride;
+          store_codes<VEC>(o + l0, x, inv);
+          store_codes<VEC>(o + l1, x + VEC, inv);
+          if (c == 0) (v ? p.sc.v : p.sc.k)[at.scale + g * p.sc.head_stride] = scale;
+        }
+      } else if (put) {
+        T* o = static_cast<T*>(v ? p.kv.v : p.kv.k) + at.values + g * p.kv.head_stride;
+        store_piece(o + l0, x);
+        store_piece(o + l1, x + VEC);
+      }
     }
+    item = next;
   }
 }
 
@@ -379,14 +379,16 @@ __global__ void __launch_bounds__(256)
 }
 
 // The vector form: heads of whole VEC-value pieces, 16 bytes of each output at a time. A thread keeps its place in the
-// rows and takes U slots, its loads of codes and scales in flight together.
+// rows and takes two slots, their loads of codes and scales in flight together (8 rows of 16384 slots of 8 x 128: 145 us,
+// 86 % of HBM; four slots 149, eight 183).
+constexpr int DEQUANT_SLOTS = 2;
 template <typename T>
 __global__ void __launch_bounds__(256)
     kv_dequant_vec_kernel(KVCache kv, KVScales sc, uint32_t n_slots, int nkv, int hd, T* __restrict__ k_out,
                           T* __restrict__ v_out, unsigned* err) {
   pdl_trigger();
   pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
-  constexpr int VEC = 16 / static_cast<int>(sizeof(T)), U = RU;
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T)), U = DEQUANT_SLOTS;
   const int lanes = hd / VEC, rows = 256 / lanes, c = threadIdx.x % lanes, i0 = threadIdx.x / lanes;
   const int64_t r = blockIdx.z, g = blockIdx.y;
   if (i0 >= rows) return;
@@ -432,12 +434,18 @@ int write_t(const WriteParams& p, bool quant, int interleaved, cudaStream_t st) 
   constexpr int PIECES = 32 / static_cast<int>(sizeof(T));   // values a lane of the vector form holds of a head
   int lanes = 1;
   while (lanes * PIECES < p.hd) lanes *= 2;
-  const unsigned groups = (p.nh + 2 * p.nkv + WHEADS - 1) / WHEADS;
-  const int64_t vec_blocks = (p.tokens * groups * lanes + 255) / 256;
-  if (write_vec_ok<T>(p, quant, interleaved) && vec_blocks < (1 << 24)) {   // thread numbers of 32 bits
-    auto kernel = quant ? (interleaved ? rotary_write_vec_kernel<T, true, true> : rotary_write_vec_kernel<T, true, false>)
-                        : (interleaved ? rotary_write_vec_kernel<T, false, true> : rotary_write_vec_kernel<T, false, false>);
-    launch_pdl_async(kernel, static_cast<unsigned>(vec_blocks), 256, 0, st, p, lanes, groups);
+  if (write_vec_ok<T>(p, quant, interleaved)) {
+    // bf16: two heads a thread and one wave of CTAs that stay (8192 tokens of 32 + 8 + 8 heads into the 8-bit cache: 35 us,
+    // 41 with a CTA for every 256 threads of work; four heads 40, 88 % of HBM to the bf16 cache). fp32 moves twice the
+    // bytes with half the arithmetic: four heads and four waves (58 us, 94 %; one wave 64).
+    constexpr int HEADS = sizeof(T) == 4 ? 4 : 2;
+    const unsigned groups = (p.nh + 2 * p.nkv + HEADS - 1) / HEADS;
+    const int64_t vec_blocks = (p.tokens * groups * lanes + 255) / 256;
+    auto kernel = quant ? (interleaved ? rotary_write_vec_kernel<T, true, true, HEADS> : rotary_write_vec_kernel<T, true, false, HEADS>)
+                        : (interleaved ? rotary_write_vec_kernel<T, false, true, HEADS> : rotary_write_vec_kernel<T, false, false, HEADS>);
+    if (vec_blocks >= 1 << 24) return fail("rotary_kv_write: too many tokens");   // 32-bit thread numbers
+    const int64_t ctas = 148 * 4 * (sizeof(T) == 4 ? 4 : 1);
+    launch_pdl_async(kernel, static_cast<unsigned>(vec_blocks < ctas ? vec_blocks : ctas), 256, 0, st, p, lanes, groups);
     return check_launch("rotary_write_vec_kernel");
   }
   const int64_t warps = p.tokens * (p.nh + 2 * p.nkv), blocks = (warps + 7) / 8;
@@ -489,7 +497,7 @@ int kv_dequant(int dtype, const KVCache& kv, const KVScales& sc, int64_t B, int6
   const uintptr_t in = reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v);
   const bool pieces = hd % vec == 0 && hd <= 256 * vec && (out & 15) == 0 && (in & (vec - 1)) == 0 &&
                       kv.block_stride % vec == 0 && kv.head_stride % vec == 0;
-  const int64_t a_block = pieces ? 256 / (hd / vec) * RU : 0;   // slots
+  const int64_t a_block = pieces ? 256 / (hd / vec) * DEQUANT_SLOTS : 0;   // slots
   const int64_t blocks = pieces ? (n_slots + a_block - 1) / a_block : (n_slots * hd + 255) / 256;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(nkv), static_cast<unsigned>(B));
   auto run = [&](auto* k, auto* v) {

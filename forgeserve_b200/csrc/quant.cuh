@@ -27,9 +27,11 @@ __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x
 // Scale of a row whose largest |x| has the bits `top`: max(|x| / 448, 2^-126); infinity and NaN stay (an fmaxf would
 // drop the NaN).
 __device__ __forceinline__ float row_scale(uint32_t top) {
-  const float s = __uint_as_float(top) / 448.f;
+  const float s = __uint_as_float(top) * (1.f / 448.f);
   return s < 1.17549435e-38f ? 1.17549435e-38f : s;
 }
+// 1 / scale, off by 2^-23 of it (scales lie in 2^-126 .. 2^120; infinity gives 0, NaN itself).
+__device__ __forceinline__ float inverse(float scale) { return __fdividef(1.f, scale); }
 
 // Two values as e4m3 codes, nearest even, saturating: lo in bits 0-7, hi in bits 8-15.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
