@@ -244,12 +244,15 @@ def paged_gather(pool: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
 
 def _row_view(t: torch.Tensor, rows: int, cols: int, name: str) -> int:
     """Row stride of t seen as `rows` rows of `cols` values; refuses other sizes and rows that overlap."""
-    n, stride = _rows(t)
-    if n != rows or t.shape[-1] != cols:
-        raise ValueError(f"{name} must hold {rows} rows of {cols} values, not {tuple(t.shape)}")
-    if n > 1 and next(t.stride(i) for i in range(t.dim() - 2, -1, -1) if t.shape[i] > 1) < cols:
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 2 and shape[0] == rows and shape[1] == cols and stride[1] == 1 and stride[0] >= cols:
+        return stride[0]
+    n, ld = _rows(t)
+    if n != rows or shape[-1] != cols:
+        raise ValueError(f"{name} must hold {rows} rows of {cols} values, not {tuple(shape)}")
+    if n > 1 and next(stride[i] for i in range(t.dim() - 2, -1, -1) if shape[i] > 1) < cols:
         raise ValueError(f"the rows of {name} overlap")
-    return stride
+    return ld
 
 
 def _check_positions(positions: torch.Tensor, n: int) -> None:
@@ -270,15 +273,29 @@ def _check_cache(kv, B: int, nkv: int, hd: int, device: torch.device, dtype: tor
     if keep is None:
         return
     k, v, table = keep[:3]
-    _on_device(device, k, v, table)
+    if k.device != device or v.device != device or table.device != device:
+        _on_device(device, k, v, table)
     if k.dtype != dtype or v.dtype != dtype:
         raise TypeError(f"the cache holds {k.dtype}, the call needs {dtype}")
-    if k.shape[1] != nkv or k.shape[3] != hd or k.shape != v.shape:
-        raise ValueError(f"the cache holds {k.shape[1]} heads of {k.shape[3]}, the call has {nkv} of {hd}")
-    if table.dtype != torch.int64 or table.numel() and table.stride(-1) != 1:
+    shape = k.shape
+    if shape[1] != nkv or shape[3] != hd or shape != v.shape:
+        raise ValueError(f"the cache holds {shape[1]} heads of {shape[3]}, the call has {nkv} of {hd}")
+    if table.dtype != torch.int64 or table.stride(-1) != 1 and table.shape[-1] > 1:
         raise ValueError("the block table must be int64 with contiguous rows")
     if table.shape[0] < B:
         raise ValueError(f"the block table has {table.shape[0]} rows, the call {B}")
+
+
+def _run(what: str, fn, device: torch.device, *args) -> None:
+    """fn(*args, stream) on the tensors' device and its current stream; raises on an error status."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        L.check(status, what)
 
 
 _ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
@@ -296,7 +313,8 @@ def rotary_kv_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optiona
     quant_paged_desc (an 8-bit cache). Returns the rotated q: q_out (B*T, nh * hd), or q's place in qkv, rotated in
     place. A negative position marks padding: its q_out row and the cache stay as they were. Two tokens of a call must
     not share a slot."""
-    require_cuda(qkv)
+    if not qkv.is_cuda:
+        require_cuda(qkv)
     dev, M = qkv.device, B * T
     ld = _row_view(qkv, M, (nh + 2 * nkv) * hd, "qkv")
     code = dtype_code(qkv.dtype)
@@ -304,14 +322,15 @@ def rotary_kv_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optiona
         raise ValueError(f"layout must be 'half' or 'interleaved', not {layout!r}")
     _check_positions(positions, M)
     _on_device(dev, positions, cos, sin, q_out)
-    rows = rd = 0
+    rows = rd = cos_p = sin_p = 0
     if cos is not None or sin is not None:
         if (cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32
                 or sin.dtype != torch.float32 or not cos.is_contiguous() or not sin.is_contiguous()):
             raise ValueError("cos and sin must be contiguous fp32 tables of one shape (positions, rotary_dim / 2)")
-        rows, rd = cos.shape[0], 2 * cos.shape[1]
+        rows, rd = cos.shape
+        rd, cos_p, sin_p = 2 * rd, cos.data_ptr(), sin.data_ptr()
     if q_out is None:
-        q_out = qkv.reshape(M, -1)[:, : nh * hd] if qkv.dim() != 2 else qkv[:, : nh * hd]
+        q_out = (qkv if qkv.dim() == 2 else qkv.view(M, -1))[:, : nh * hd]
         ldq = ld
     else:
         if q_out.dtype != qkv.dtype:
@@ -320,25 +339,23 @@ def rotary_kv_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optiona
     quant = isinstance(kv, L.KVQuantDesc)
     _check_cache(kv, B, nkv, hd, dev, torch.float8_e4m3fn if quant else qkv.dtype)
     lib = L.load()
-    with torch.cuda.device(dev):
-        L.check((lib.fs_rotary_kv_write_quant if quant else lib.fs_rotary_kv_write)(
-            _p(qkv), ld, _p(q_out), ldq, _p(cos), _p(sin), rows, rd, _ROPE_LAYOUTS[layout], _p(positions),
-            ctypes.byref(kv), B, T, nh, nkv, hd, slot_base, int(slot_from_pos), code, _stream(qkv)),
-            "fs_rotary_kv_write")
+    _run("fs_rotary_kv_write", lib.fs_rotary_kv_write_quant if quant else lib.fs_rotary_kv_write, dev,
+         qkv.data_ptr(), ld, q_out.data_ptr(), ldq, cos_p, sin_p, rows, rd, _ROPE_LAYOUTS[layout], positions.data_ptr(),
+         kv, B, T, nh, nkv, hd, slot_base, slot_from_pos, code)
     return q_out
 
 
 def kv_dequant(kv: L.KVQuantDesc, B: int, n_slots: int, nkv: int, hd: int, dtype: torch.dtype):
     """The first n_slots slots of every row of an 8-bit cache as dense (k, v), each (B, nkv, n_slots, hd) of dtype."""
-    dev = kv.keep[0].device
-    require_cuda(kv.keep[0])
+    codes = kv.keep[0]
+    if not codes.is_cuda:
+        require_cuda(codes)
+    dev = codes.device
     code = dtype_code(dtype)
     _check_cache(kv, B, nkv, hd, dev, torch.float8_e4m3fn)
-    k = torch.empty(B, nkv, n_slots, hd, dtype=dtype, device=dev)
+    k = torch.empty((B, nkv, n_slots, hd), dtype=dtype, device=dev)
     v = torch.empty_like(k)
-    with torch.cuda.device(dev):
-        L.check(L.load().fs_kv_dequant(ctypes.byref(kv), B, n_slots, nkv, hd, _p(k), _p(v), code, _stream(k)),
-                "fs_kv_dequant")
+    _run("fs_kv_dequant", L.load().fs_kv_dequant, dev, kv, B, n_slots, nkv, hd, k.data_ptr(), v.data_ptr(), code)
     return k, v
 
 
@@ -346,7 +363,8 @@ def attention_decode_quant(q: torch.Tensor, kv: L.KVQuantDesc, n_slots: int, pos
                            out: torch.Tensor, B: int, nh: int, nkv: int, hd: int) -> torch.Tensor:
     """attention_decode over an 8-bit cache: one query per row (positions (B,) or (B, 1)), any n_heads / n_kv_heads,
     even head_dim up to 256. A row with a negative position sees no slot and gets zeros."""
-    require_cuda(q)
+    if not q.is_cuda:
+        require_cuda(q)
     dev = q.device
     _on_device(dev, positions, out)
     if out.dtype != q.dtype:
@@ -356,13 +374,12 @@ def attention_decode_quant(q: torch.Tensor, kv: L.KVQuantDesc, n_slots: int, pos
     _check_positions(positions, B)
     _check_cache(kv, B, nkv, hd, dev, torch.float8_e4m3fn)
     lib = L.load()
-    need = lib.fs_attention_decode_quant_workspace(B, nh, nkv, hd, n_slots)
     # Allocated by each call: the allocator hands it out in stream order, and a captured call's stays with its graph.
+    need = lib.fs_attention_decode_quant_workspace(B, nh, nkv, hd, n_slots)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    with torch.cuda.device(dev):
-        L.check(lib.fs_attention_decode_quant(_p(q), ldq, ctypes.byref(kv), n_slots, _p(positions), _p(out), ldo, B, nh,
-                                              nkv, hd, 1.0 / math.sqrt(hd), _p(ws), need, code, _stream(q)),
-                "fs_attention_decode_quant")
+    _run("fs_attention_decode_quant", lib.fs_attention_decode_quant, dev, q.data_ptr(), ldq, kv, n_slots,
+         positions.data_ptr(), out.data_ptr(), ldo, B, nh, nkv, hd, 1.0 / math.sqrt(hd),
+         0 if ws is None else ws.data_ptr(), need, code)
     return out
 
 
@@ -410,21 +427,20 @@ def quant_paged_desc(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_
                      table: torch.Tensor) -> L.KVQuantDesc:
     """Descriptor of an 8-bit paged pool: codes k, v float8_e4m3fn (num_blocks, nkv, block_size, hd), scales fp32
     (num_blocks, nkv, block_size); table (B, nb) int64."""
-    nblk, nkv, bs, hd = k.shape
+    shape, strides, rows, cols = k.shape, k.stride(), k_scale.shape, k_scale.stride()
     if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
         raise TypeError("quant_paged_desc: k and v must be float8_e4m3fn")
     if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
         raise TypeError("quant_paged_desc: the scales must be float32")
-    if v.shape != k.shape or k_scale.shape != k.shape[:3] or v_scale.shape != k.shape[:3]:
+    if len(shape) != 4 or v.shape != shape or rows != shape[:3] or v_scale.shape != rows:
         raise ValueError("quant_paged_desc: k, v and their scales must describe one pool")
-    s0, s1, s2, s3 = k.stride()
-    c0, c1, c2 = k_scale.stride()
-    if v.stride() != k.stride() or v_scale.stride() != k_scale.stride() or (s2, s3, c2) != (hd, 1, 1):
+    if (v.stride() != strides or v_scale.stride() != cols or strides[3] != 1 or strides[2] != shape[3] or cols[2] != 1
+            or min(strides[:2]) < 0 or min(cols[:2]) < 0):
         raise ValueError("quant_paged_desc: the slots of a (block, head) must lie contiguously, k and v alike")
     if table.dim() != 2:
         raise ValueError("quant_paged_desc: the block table must be 2-D")
     _on_device(k.device, v, k_scale, v_scale, table)
-    desc = L.KVQuantDesc(L.KVCacheDesc(k.data_ptr(), v.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], bs,
-                                       s0, s1, nblk), k_scale.data_ptr(), v_scale.data_ptr(), c0, c1)
+    desc = L.KVQuantDesc((k.data_ptr(), v.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], shape[2],
+                          strides[0], strides[1], shape[0]), k_scale.data_ptr(), v_scale.data_ptr(), cols[0], cols[1])
     desc.keep = (k, v, table, k_scale, v_scale)
     return desc
