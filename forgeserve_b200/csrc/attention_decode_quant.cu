@@ -64,7 +64,7 @@ __device__ __forceinline__ int64_t visible(const Params& p, int64_t r) {
 // max that an exponent may be taken against: -infinity (no finite score) becomes 0, so that exp2(-inf - m) is 0.
 __device__ __forceinline__ float safe_max(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Any type, hd (<= 256) and layout: 32 keys at a time as fp32 in shared memory; a warp owns two query heads, a lane
+// What the tensor-core kernel below does not take (hd no multiple of 16, rows off 16 bytes): any hd <= 256 and layout, 32 keys at a time as fp32 in shared memory; a warp owns two query heads, a lane
 // one key of the scores and hd / 32 dims of the sums.
 template <typename T>
 __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
@@ -171,7 +171,8 @@ __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
 }
 
 // ------------------------------------------------------------------------------------ tensor-core kernel
-// hd 64, 128 or 256, 16-byte rows. The codes are exact in f16, so both products run as mma.sync m16n8k16 f16 with fp32
+// hd a multiple of 16 up to 256, 16-byte rows; the kernel is built for HD = 64, 128 and 256, dims from hd on are zeros in
+// shared memory (no bytes of the cache). The codes are exact in f16, so both products run as mma.sync m16n8k16 f16 with fp32
 // sums and the scales never touch them; the query heads of the KV head are the N side (NT tiles of 8):
 //     S^T (16 keys x 8 heads) = K (16 x hd) Q^T (hd x 8),   O^T (hd x 8 heads) += V^T (hd x 16) P^T (16 x 8)
 // A contraction's index order is free as long as both operands agree, and so are the rows of O^T; they are chosen so
@@ -351,8 +352,8 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
   const int64_t n_vis = visible(p, r), per = split_keys(n_vis, p.nkv), begin = split * per;
   if (begin >= n_vis) {
     if (p.splits == 1)   // a row that sees nothing
-      for (int i = threadIdx.x; i < heads * HD; i += blockDim.x)
-        static_cast<T*>(p.out)[r * p.ldo + static_cast<int64_t>(kvh * p.rep + h0) * HD + i] = from_f<T>(0.f);
+      for (int i = threadIdx.x; i < heads * p.hd; i += blockDim.x)
+        static_cast<T*>(p.out)[r * p.ldo + static_cast<int64_t>(kvh * p.rep + h0) * p.hd + i] = from_f<T>(0.f);
     return;              // the join does not read an empty split
   }
   const int n_keys = static_cast<int>(n_vis - begin < per ? n_vis - begin : per);
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
           const int64_t blk = col < p.kv.table_cols ? p.kv.table[r * p.kv.table_stride + col] : -1;
           if (blk >= 0 && blk < p.kv.num_blocks) {
             a = WHOLE ? blk * p.rows_per_block + kvh * p.rows_per_head + in
-                      : blk * p.kv.block_stride + kvh * p.kv.head_stride + in * HD;
+                      : blk * p.kv.block_stride + kvh * p.kv.head_stride + in * p.hd;
             b = blk * p.sc.block_stride + kvh * p.sc.head_stride + in;
           } else {
             flag_error(p.err, ERR_BAD_SLOT);
@@ -419,8 +420,11 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
         const int64_t o = a[gl + 8 * i];
         const uint8_t* src = o >= 0 ? static_cast<const uint8_t*>(p.kv.k) + o : none;
 #pragma unroll
-        for (int c = 0; c < G::KC; ++c)
-          copy_async<16>(smem_u32(buf) + ((i * G::KC + c) * 32 + lane) * 16, src + k_chunk<HD, WHOLE>(tl, c) * 16, o >= 0);
+        for (int c = 0; c < G::KC; ++c) {
+          const int d = k_chunk<HD, WHOLE>(tl, c) * 16;
+          copy_async<16>(smem_u32(buf) + ((i * G::KC + c) * 32 + lane) * 16, d < p.hd ? src + d : none,
+                         o >= 0 && d < p.hd);
+        }
       }
     }
   };
@@ -434,9 +438,11 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
         const int64_t o = a[(i >> 2) * TILE + 2 * tl + (i & 1) + 4 * (i & 2)];
         const uint8_t* src = o >= 0 ? static_cast<const uint8_t*>(p.kv.v) + o : none;
 #pragma unroll
-        for (int c = 0; c < G::VC; ++c)
+        for (int c = 0; c < G::VC; ++c) {
+          const int d = c * 128 + gl * G::VB;
           copy_async<G::VB>(smem_u32(buf) + G::STEP_BYTES + ((i * G::VC + c) * 32 + lane) * G::VB,
-                            src + c * 128 + gl * G::VB, o >= 0);
+                            d < p.hd ? src + d : none, o >= 0 && d < p.hd);
+        }
       }
     }
   };
@@ -479,12 +485,20 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
   for (int n = 0; n < NT; ++n) {
     const bool real = 8 * n + gl < heads;
     const T* q = static_cast<const T*>(p.q) + r * p.ldq +
-                 static_cast<int64_t>(kvh * p.rep + h0 + (real ? 8 * n + gl : 0)) * HD;
+                 static_cast<int64_t>(kvh * p.rep + h0 + (real ? 8 * n + gl : 0)) * p.hd;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int WORDS = F32 ? 16 : 8;   // of 16 values
     uint32_t x[G::KC * WORDS], top = 0;
 #pragma unroll
-    for (int c = 0; c < G::KC; ++c) load16(q + k_chunk<HD, WHOLE>(tl, c) * 16, p.q_vec, x + c * WORDS);
+    for (int c = 0; c < G::KC; ++c) {
+      const int d = k_chunk<HD, WHOLE>(tl, c) * 16;
+      if (d < p.hd) {
+        load16(q + d, p.q_vec, x + c * WORDS);
+      } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) x[c * WORDS + i] = 0;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < G::KC * WORDS; ++i)
       top = F32 ? max(top, x[i] & 0x7fffffffu) : __vmaxu2(top, x[i] & 0x7fff7fffu);
@@ -775,7 +789,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) wsm[h * WARPS + w] = p.splits == 1 ? f[w] / total : f[w];
     if (p.splits > 1) {
-      float* ml = p.ws + static_cast<int64_t>(gridDim.z) * p.nh * p.splits * HD +
+      float* ml = p.ws + static_cast<int64_t>(gridDim.z) * p.nh * p.splits * p.hd +
                   2 * (part0 + static_cast<int64_t>(h) * p.splits);
       ml[0] = top;
       ml[1] = total;
@@ -784,6 +798,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
   __syncthreads();
   for (int i = threadIdx.x * 4; i < heads * HD; i += blockDim.x * 4) {
     const int h = i / HD, d = i % HD;
+    if (d >= p.hd) continue;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
@@ -795,19 +810,19 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
       o.w = fmaf(f, x.w, o.w);
     }
     if (p.splits == 1) {
-      T* dst = static_cast<T*>(p.out) + r * p.ldo + static_cast<int64_t>(kvh * p.rep + h0 + h) * HD + d;
+      T* dst = static_cast<T*>(p.out) + r * p.ldo + static_cast<int64_t>(kvh * p.rep + h0 + h) * p.hd + d;
       dst[0] = from_f<T>(o.x);
       dst[1] = from_f<T>(o.y);
       dst[2] = from_f<T>(o.z);
       dst[3] = from_f<T>(o.w);
     } else {
-      *reinterpret_cast<float4*>(p.ws + (part0 + static_cast<int64_t>(h) * p.splits) * HD + d) = o;
+      *reinterpret_cast<float4*>(p.ws + (part0 + static_cast<int64_t>(h) * p.splits) * p.hd + d) = o;
     }
   }
 }
 
 bool supported(const Params& p) {
-  if (p.hd != 64 && p.hd != 128 && p.hd != 256) return false;
+  if (p.hd % 16 || p.hd > 256) return false;
   return p.kv.block_stride % 16 == 0 && p.kv.head_stride % 16 == 0 &&
          ((reinterpret_cast<uintptr_t>(p.kv.k) | reinterpret_cast<uintptr_t>(p.kv.v)) & 15) == 0;
 }
@@ -827,10 +842,10 @@ int launch_geo(Params p, int64_t B, int64_t nkv, cudaStream_t st) {
   if (nkv * p.groups > 65535) return fail("fs_attention_decode_quant: too many heads");
   CUtensorMap mk = {}, mv = {};
   if constexpr (WHOLE) {
-    p.rows_per_block = static_cast<int>(p.kv.block_stride / HD);
-    p.rows_per_head = static_cast<int>(p.kv.head_stride / HD);
+    p.rows_per_block = static_cast<int>(p.kv.block_stride / p.hd);
+    p.rows_per_head = static_cast<int>(p.kv.head_stride / p.hd);
     p.map_rows = static_cast<int>((p.kv.num_blocks - 1) * p.rows_per_block + (nkv - 1) * p.rows_per_head + p.kv.block_size);
-    if (make_byte_map(&mk, p.kv.k, HD, p.map_rows, TILE) || make_byte_map(&mv, p.kv.v, HD, p.map_rows, TILE)) return -1;
+    if (make_byte_map(&mk, p.kv.k, p.hd, p.map_rows, TILE) || make_byte_map(&mv, p.kv.v, p.hd, p.map_rows, TILE)) return -1;
   }
   static bool attr[64] = {false};
   int dev = 0;
@@ -856,8 +871,8 @@ int launch_hd(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
 
 template <typename T>
 int launch_t(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
-  return p.hd == 64 ? launch_hd<T, 64>(p, B, nkv, st)
-                    : p.hd == 128 ? launch_hd<T, 128>(p, B, nkv, st) : launch_hd<T, 256>(p, B, nkv, st);
+  return p.hd <= 64 ? launch_hd<T, 64>(p, B, nkv, st)
+                    : p.hd <= 128 ? launch_hd<T, 128>(p, B, nkv, st) : launch_hd<T, 256>(p, B, nkv, st);
 }
 
 }  // namespace tc

@@ -105,8 +105,8 @@ __device__ __forceinline__ void flag_error(unsigned* err, unsigned code) {
 // 2-D bf16 tensor map with 128-byte swizzle and boxes of 64 columns x box_rows rows, over a row-major matrix of
 // `rows` rows of `cols` elements at a stride of `ld` elements (defined in attention_tc.cu).
 int make_bf16_map(CUtensorMap* map, const void* ptr, int64_t cols, int64_t rows, int64_t ld, int box_rows);
-// 2-D byte tensor map over `rows` contiguous rows of `cols` (64, or a multiple of 128) bytes, boxes of one row's width up
-// to 128 bytes x box_rows rows, swizzled over that width.
+// 2-D byte tensor map over `rows` contiguous rows of `cols` bytes (a multiple of 16), boxes of 64 bytes (rows of up to 64)
+// or 128 x box_rows rows, swizzled over that width; bytes past a row's end read as zeros.
 int make_byte_map(CUtensorMap* map, const void* ptr, int64_t cols, int64_t rows, int box_rows);
 
 // ---------------------------------------------------------------------------------------------------------

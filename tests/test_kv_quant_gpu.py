@@ -173,7 +173,7 @@ def test_rotary_write_contiguous_cache_and_strided_rows():
             assert not k[:, :, :base].any() and not k[:, :, base + T:].any()
 
 
-@pytest.mark.parametrize("hd", [128, 80])
+@pytest.mark.parametrize("hd", [128, 80, 18])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_store_special_rows(dtype, hd):
     """Rows of zeros, of the smallest and largest values, with an infinity, with a NaN; each alone in its row."""
@@ -339,6 +339,18 @@ DECODE_CASES = [  # dtype, lengths, nh, nkv, hd, bs
     (torch.float32, [640, 30], 9, 1, 256, 48),
     (torch.float32, [640, 30], 4, 2, 96, 16),
     (torch.float32, [70], 3, 3, 6, 2),
+    # head sizes between the ones that the tensor-core kernel is built for
+    (torch.bfloat16, [100, 523, 31, 0], 8, 2, 16, 16),
+    (torch.bfloat16, [100, 523, 31, 0], 8, 2, 48, 10),
+    (torch.bfloat16, [100, 523, 31, 0], 18, 2, 96, 32),
+    (torch.bfloat16, [100, 523, 31, 0], 8, 2, 112, 16),
+    (torch.bfloat16, [100, 523, 31, 0], 8, 2, 144, 16),
+    (torch.bfloat16, [100, 523, 31, 0], 8, 2, 192, 9),
+    (torch.bfloat16, [100, 523, 31, 0], 20, 2, 240, 16),
+    (torch.float32, [100, 523, 31, 0], 8, 2, 80, 16),
+    (torch.float32, [100, 523, 31, 0], 20, 2, 208, 16),
+    (torch.float32, [100, 523, 31, 0], 8, 2, 32, 3),
+    (torch.bfloat16, [100, 523, 31, 0], 8, 2, 40, 16),
     # rows long enough for splits of several units of 512 slots, beside short ones
     (torch.bfloat16, [19000, 700, 9500, 4700], 64, 64, 64, 16),
     (torch.bfloat16, [11000, 513, 5000], 256, 128, 128, 24),
@@ -358,7 +370,8 @@ def test_decode(case):
 
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd", [(torch.bfloat16, 8, 2, 128), (torch.float32, 8, 2, 128),
-                                             (torch.bfloat16, 4, 2, 80)])
+                                             (torch.bfloat16, 4, 2, 80), (torch.bfloat16, 4, 2, 40),
+                                             (torch.float32, 4, 1, 256)])
 def test_decode_does_not_read_past_the_visible_slots(dtype, nh, nkv, hd):
     """NaN scales and codes behind each row's last slot, in unused blocks and past n_slots change nothing."""
     lengths = [1, 15, 530, 517]
@@ -381,7 +394,7 @@ def test_decode_does_not_read_past_the_visible_slots(dtype, nh, nkv, hd):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("hd", [128, 80])
+@pytest.mark.parametrize("hd", [128, 80, 40])
 def test_decode_special_values(dtype, hd):
     """NaN and infinity in a visible key or value reach their row and KV head only; rows of zero scale, queries far out
     of the half range, values whose scales span many powers of two."""
@@ -481,7 +494,7 @@ def test_decode_is_independent_of_batch_and_table_width():
 
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd,bs", [(torch.bfloat16, 32, 4, 128, 16), (torch.float32, 32, 16, 64, 16),
-                                                (torch.bfloat16, 32, 8, 128, 20), (torch.bfloat16, 32, 8, 80, 16)])
+                                                (torch.bfloat16, 32, 8, 128, 20), (torch.bfloat16, 32, 8, 40, 16)])
 def test_decode_bits_do_not_depend_on_the_batch(dtype, nh, nkv, hd, bs):
     """Rows of a batch large enough for another join, and behind a table of other width, against each row alone."""
     lengths = [1 + (i * 797) % 3000 for i in range(40)]
