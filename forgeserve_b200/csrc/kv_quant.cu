@@ -378,53 +378,43 @@ __global__ void __launch_bounds__(256)
   v_out[o] = from_f<T>(v);
 }
 
-// The vector form: heads of whole VEC-value pieces, 16 bytes of each output at a time. A thread keeps its place in the
-// rows and takes two slots, their loads of codes and scales in flight together (8 rows of 16384 slots of 8 x 128: 145 us,
-// 86 % of HBM; four slots 149, eight 183).
-constexpr int DEQUANT_SLOTS = 2;
+// The vector form: heads of whole VEC-value pieces, 16 bytes of each output at a time. One wave of CTAs stays and takes
+// chunks of 256 / (hd / VEC) slots of a (row, head) in turn; many small CTAs an SM (8) beat more loads a thread (8 rows of
+// 16384 slots of 8 x 128: 139 us, 89 % of HBM; two slots a thread 141 at 6 CTAs, a CTA for every chunk 165).
+constexpr int DEQUANT_CTAS = 8;
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, DEQUANT_CTAS)
     kv_dequant_vec_kernel(KVCache kv, KVScales sc, uint32_t n_slots, int nkv, int hd, T* __restrict__ k_out,
-                          T* __restrict__ v_out, unsigned* err) {
+                          T* __restrict__ v_out, unsigned* err, unsigned chunks, unsigned total) {
   pdl_trigger();
   pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
-  constexpr int VEC = 16 / static_cast<int>(sizeof(T)), U = DEQUANT_SLOTS;
-  const int lanes = hd / VEC, rows = 256 / lanes, c = threadIdx.x % lanes, i0 = threadIdx.x / lanes;
-  const int64_t r = blockIdx.z, g = blockIdx.y;
-  if (i0 >= rows) return;
-  const uint32_t s0 = blockIdx.x * (rows * U) + i0;
-  uint2 ck[U], cv[U];
-  float sk[U], sv[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t s = s0 + u * rows;
-    ck[u] = cv[u] = make_uint2(0, 0);
-    sk[u] = sv[u] = 0.f;
-    if (s < n_slots) {
-      int64_t col, in;
-      split_slot(s, kv.block_size, col, in);
-      const int64_t blk = col < kv.table_cols ? kv.table[r * kv.table_stride + col] : -1;
-      if (blk >= 0 && blk < kv.num_blocks) {
-        const int64_t at = blk * kv.block_stride + g * kv.head_stride + in * hd + c * VEC;
-        const int64_t sat = blk * sc.block_stride + g * sc.head_stride + in;
-        ck[u] = load_codes<VEC>(static_cast<const uint8_t*>(kv.k) + at);
-        cv[u] = load_codes<VEC>(static_cast<const uint8_t*>(kv.v) + at);
-        sk[u] = sc.k[sat];
-        sv[u] = sc.v[sat];
-      } else if (c == 0 && in == 0) {
-        flag_error(err, ERR_BAD_SLOT);
-      }
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+  const int lanes = hd / VEC, rows = 256 / lanes, c = threadIdx.x % lanes, i = threadIdx.x / lanes;
+  if (i >= rows) return;
+  for (unsigned item = blockIdx.x; item < total; item += gridDim.x) {
+    const unsigned rg = item / chunks, r = rg / nkv, g = rg - r * nkv;
+    const uint32_t s = (item - rg * chunks) * rows + i;
+    if (s >= n_slots) continue;
+    int64_t col, in;
+    split_slot(s, kv.block_size, col, in);
+    const int64_t blk = col < kv.table_cols ? kv.table[r * kv.table_stride + col] : -1;
+    uint2 ck = make_uint2(0, 0), cv = ck;
+    float sk = 0.f, sv = 0.f;
+    if (blk >= 0 && blk < kv.num_blocks) {
+      const int64_t at = blk * kv.block_stride + g * kv.head_stride + in * hd + c * VEC;
+      const int64_t sat = blk * sc.block_stride + g * sc.head_stride + in;
+      ck = load_codes<VEC>(static_cast<const uint8_t*>(kv.k) + at);
+      cv = load_codes<VEC>(static_cast<const uint8_t*>(kv.v) + at);
+      sk = sc.k[sat];
+      sv = sc.v[sat];
+    } else if (c == 0 && in == 0) {
+      flag_error(err, ERR_BAD_SLOT);
     }
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t s = s0 + u * rows;
-    if (s >= n_slots) break;
-    const int64_t o = ((r * nkv + g) * n_slots + s) * hd + c * VEC;
+    const int64_t o = (static_cast<int64_t>(rg) * n_slots + s) * hd + c * VEC;
     float x[VEC];
-    decode_piece<VEC>(ck[u], sk[u], x);
+    decode_piece<VEC>(ck, sk, x);
     store_piece(k_out + o, x);
-    decode_piece<VEC>(cv[u], sv[u], x);
+    decode_piece<VEC>(cv, sv, x);
     store_piece(v_out + o, x);
   }
 }
@@ -497,13 +487,25 @@ int kv_dequant(int dtype, const KVCache& kv, const KVScales& sc, int64_t B, int6
   const uintptr_t in = reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v);
   const bool pieces = hd % vec == 0 && hd <= 256 * vec && (out & 15) == 0 && (in & (vec - 1)) == 0 &&
                       kv.block_stride % vec == 0 && kv.head_stride % vec == 0;
-  const int64_t a_block = pieces ? 256 / (hd / vec) * DEQUANT_SLOTS : 0;   // slots
-  const int64_t blocks = pieces ? (n_slots + a_block - 1) / a_block : (n_slots * hd + 255) / 256;
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(nkv), static_cast<unsigned>(B));
+  if (pieces) {
+    const int64_t rows = 256 / (hd / vec), chunks = (n_slots + rows - 1) / rows, total = chunks * B * nkv;
+    if (total > INT32_MAX) return fail("fs_kv_dequant: too many slots");
+    const unsigned ctas = static_cast<unsigned>(total < 148 * DEQUANT_CTAS ? total : 148 * DEQUANT_CTAS);
+    if (dtype == F32)
+      launch_pdl_async(kv_dequant_vec_kernel<float>, ctas, 256, 0, st, kv, sc, static_cast<uint32_t>(n_slots),
+                       static_cast<int>(nkv), static_cast<int>(hd), static_cast<float*>(k_out),
+                       static_cast<float*>(v_out), err, static_cast<unsigned>(chunks), static_cast<unsigned>(total));
+    else
+      launch_pdl_async(kv_dequant_vec_kernel<__nv_bfloat16>, ctas, 256, 0, st, kv, sc, static_cast<uint32_t>(n_slots),
+                       static_cast<int>(nkv), static_cast<int>(hd), static_cast<__nv_bfloat16*>(k_out),
+                       static_cast<__nv_bfloat16*>(v_out), err, static_cast<unsigned>(chunks), static_cast<unsigned>(total));
+    return check_launch("kv_dequant_vec_kernel");
+  }
+  const dim3 grid(static_cast<unsigned>((n_slots * hd + 255) / 256), static_cast<unsigned>(nkv), static_cast<unsigned>(B));
   auto run = [&](auto* k, auto* v) {
     using T = std::remove_pointer_t<decltype(k)>;
-    launch_pdl_async(pieces ? kv_dequant_vec_kernel<T> : kv_dequant_kernel<T>, grid, 256, 0, st, kv, sc,
-                     static_cast<uint32_t>(n_slots), static_cast<int>(nkv), static_cast<int>(hd), k, v, err);
+    launch_pdl_async(kv_dequant_kernel<T>, grid, 256, 0, st, kv, sc, static_cast<uint32_t>(n_slots),
+                     static_cast<int>(nkv), static_cast<int>(hd), k, v, err);
   };
   if (dtype == F32)
     run(static_cast<float*>(k_out), static_cast<float*>(v_out));

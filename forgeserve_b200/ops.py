@@ -4,6 +4,7 @@ pointers and the caller's current CUDA stream to libforgeserve_b200.so, and retu
 
 import ctypes
 import math
+import struct
 from typing import List, Optional
 
 import torch
@@ -272,7 +273,7 @@ def _check_cache(kv, B: int, nkv: int, hd: int, device: torch.device, dtype: tor
     keep = getattr(kv, "keep", None)
     if keep is None:
         return
-    k, v, table = keep[:3]
+    k, v, table = keep[0], keep[1], keep[2]
     if k.device != device or v.device != device or table.device != device:
         _on_device(device, k, v, table)
     if k.dtype != dtype or v.dtype != dtype:
@@ -280,10 +281,19 @@ def _check_cache(kv, B: int, nkv: int, hd: int, device: torch.device, dtype: tor
     shape = k.shape
     if shape[1] != nkv or shape[3] != hd or shape != v.shape:
         raise ValueError(f"the cache holds {shape[1]} heads of {shape[3]}, the call has {nkv} of {hd}")
-    if table.dtype != torch.int64 or table.stride(-1) != 1 and table.shape[-1] > 1:
+    if table.dim() > 2 or table.dtype != torch.int64 or table.stride(-1) != 1 and table.shape[-1] > 1:
         raise ValueError("the block table must be int64 with contiguous rows")
     if table.shape[0] < B:
         raise ValueError(f"the block table has {table.shape[0]} rows, the call {B}")
+
+
+def _check_quant_cache(kv: L.KVQuantDesc, B: int, nkv: int, hd: int, device: torch.device) -> None:
+    """A quant_paged_desc against a call's sizes (its tensors were checked against each other when it was made)."""
+    about = getattr(kv, "about", None)
+    if about is not None and (about[0] != device or about[1] != nkv or about[2] != hd or about[3] < B):
+        _on_device(device, kv.keep[0])
+        raise ValueError(f"the cache holds {about[1]} heads of {about[2]} for {about[3]} rows, the call has {nkv} of {hd} "
+                         f"for {B}")
 
 
 def _run(what: str, fn, device: torch.device, *args) -> None:
@@ -337,7 +347,10 @@ def rotary_kv_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optiona
             raise TypeError("q_out must have qkv's dtype")
         ldq = _row_view(q_out, M, nh * hd, "q_out") if nh else 0
     quant = isinstance(kv, L.KVQuantDesc)
-    _check_cache(kv, B, nkv, hd, dev, torch.float8_e4m3fn if quant else qkv.dtype)
+    if quant:
+        _check_quant_cache(kv, B, nkv, hd, dev)
+    else:
+        _check_cache(kv, B, nkv, hd, dev, qkv.dtype)
     lib = L.load()
     _run("fs_rotary_kv_write", lib.fs_rotary_kv_write_quant if quant else lib.fs_rotary_kv_write, dev,
          qkv.data_ptr(), ld, q_out.data_ptr(), ldq, cos_p, sin_p, rows, rd, _ROPE_LAYOUTS[layout], positions.data_ptr(),
@@ -352,7 +365,7 @@ def kv_dequant(kv: L.KVQuantDesc, B: int, n_slots: int, nkv: int, hd: int, dtype
         require_cuda(codes)
     dev = codes.device
     code = dtype_code(dtype)
-    _check_cache(kv, B, nkv, hd, dev, torch.float8_e4m3fn)
+    _check_quant_cache(kv, B, nkv, hd, dev)
     k = torch.empty((B, nkv, n_slots, hd), dtype=dtype, device=dev)
     v = torch.empty_like(k)
     _run("fs_kv_dequant", L.load().fs_kv_dequant, dev, kv, B, n_slots, nkv, hd, k.data_ptr(), v.data_ptr(), code)
@@ -372,7 +385,7 @@ def attention_decode_quant(q: torch.Tensor, kv: L.KVQuantDesc, n_slots: int, pos
     code = dtype_code(q.dtype)
     ldq, ldo = _row_view(q, B, nh * hd, "q"), _row_view(out, B, nh * hd, "out")
     _check_positions(positions, B)
-    _check_cache(kv, B, nkv, hd, dev, torch.float8_e4m3fn)
+    _check_quant_cache(kv, B, nkv, hd, dev)
     lib = L.load()
     # Allocated by each call: the allocator hands it out in stream order, and a captured call's stays with its graph.
     need = lib.fs_attention_decode_quant_workspace(B, nh, nkv, hd, n_slots)
@@ -423,24 +436,37 @@ def paged_desc(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> L.KVCac
     return desc
 
 
+_PACK_QUANT = struct.Struct("13q").pack   # the fields of KVQuantDesc, all 8 bytes
+
+
 def quant_paged_desc(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                      table: torch.Tensor) -> L.KVQuantDesc:
     """Descriptor of an 8-bit paged pool: codes k, v float8_e4m3fn (num_blocks, nkv, block_size, hd), scales fp32
     (num_blocks, nkv, block_size); table (B, nb) int64."""
-    shape, strides, rows, cols = k.shape, k.stride(), k_scale.shape, k_scale.stride()
     if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
         raise TypeError("quant_paged_desc: k and v must be float8_e4m3fn")
     if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
         raise TypeError("quant_paged_desc: the scales must be float32")
-    if len(shape) != 4 or v.shape != shape or rows != shape[:3] or v_scale.shape != rows:
+    if k.dim() != 4 or table.dim() != 2:
+        raise ValueError("quant_paged_desc: k and v must be 4-D, the block table 2-D")
+    nblk, nkv, bs, hd = shape = k.shape
+    rows = (nblk, nkv, bs)
+    if v.shape != shape or k_scale.shape != rows or v_scale.shape != rows:
         raise ValueError("quant_paged_desc: k, v and their scales must describe one pool")
-    if (v.stride() != strides or v_scale.stride() != cols or strides[3] != 1 or strides[2] != shape[3] or cols[2] != 1
-            or min(strides[:2]) < 0 or min(cols[:2]) < 0):
+    s0, s1, s2, s3 = strides = k.stride()
+    c0, c1, c2 = cols = k_scale.stride()
+    if (v.stride() != strides or v_scale.stride() != cols or s3 != 1 or s2 != hd or c2 != 1
+            or s0 < 0 or s1 < 0 or c0 < 0 or c1 < 0):
         raise ValueError("quant_paged_desc: the slots of a (block, head) must lie contiguously, k and v alike")
-    if table.dim() != 2:
-        raise ValueError("quant_paged_desc: the block table must be 2-D")
-    _on_device(k.device, v, k_scale, v_scale, table)
-    desc = L.KVQuantDesc((k.data_ptr(), v.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], shape[2],
-                          strides[0], strides[1], shape[0]), k_scale.data_ptr(), v_scale.data_ptr(), cols[0], cols[1])
+    (n, width), (t0, t1) = table.shape, table.stride()
+    if table.dtype != torch.int64 or t1 != 1 and width > 1:
+        raise ValueError("the block table must be int64 with contiguous rows")
+    dev = k.device
+    if v.device != dev or k_scale.device != dev or v_scale.device != dev or table.device != dev:
+        _on_device(dev, v, k_scale, v_scale, table)
+    desc = L.KVQuantDesc.from_buffer_copy(_PACK_QUANT(
+        k.data_ptr(), v.data_ptr(), table.data_ptr(), t0, width, bs, s0, s1, nblk, k_scale.data_ptr(), v_scale.data_ptr(),
+        c0, c1))
     desc.keep = (k, v, table, k_scale, v_scale)
+    desc.about = (dev, nkv, hd, n)
     return desc
