@@ -899,13 +899,28 @@ __global__ void __launch_bounds__(128) quant_combine_kernel(Params p) {
   const float2* src = reinterpret_cast<const float2*>(p.ws + base * hd);
   T* dst = static_cast<T*>(p.out) + r * p.ldo + (id - r * p.nh) * hd;
   float* w = weights[team];
-  float top = -INFINITY, total = 0.f;
-  for (int s = lane; s < used; s += 32) top = fmaxf(top, ml[s].x);
+  // W = 4: the first splits' values are asked for before their number is known (the workspace holds p.splits of each)
+  constexpr int EARLY = W == 1 ? 1 : 4;
+  float2 early[EARLY][2];
+  if constexpr (W == 4) {
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) {
+      const int s = warp + 4 * i;
+      early[i][0] = early[i][1] = make_float2(0.f, 0.f);
+      if (s < p.splits) {
+        if (lane < cols) early[i][0] = src[static_cast<int64_t>(s) * cols + lane];
+        if (lane + 32 < cols) early[i][1] = src[static_cast<int64_t>(s) * cols + lane + 32];
+      }
+    }
+  }
+  const float2 first = lane < p.splits ? ml[lane] : make_float2(0.f, 0.f);
+  float top = lane < used ? first.x : -INFINITY, total = 0.f;
+  for (int s = lane + 32; s < used; s += 32) top = fmaxf(top, ml[s].x);
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
   top = safe_max(top);
   for (int s = lane; s < used; s += 32) {
-    const float2 v = ml[s];
+    const float2 v = s < 32 ? first : ml[s];
     const float f = exp2f(v.x - top);
     total = fmaf(f, v.y, total);
     if (W == 1 || warp == 0) w[s] = f;
@@ -919,25 +934,27 @@ __global__ void __launch_bounds__(128) quant_combine_kernel(Params p) {
     float2 a[SUMS], b[SUMS];
 #pragma unroll
     for (int g = 0; g < SUMS; ++g) a[g] = b[g] = make_float2(0.f, 0.f);
-#pragma unroll(W == 1 ? 2 : 8)
-    for (int s0 = W == 1 ? 0 : warp; s0 < used; s0 += 4) {
+    auto add = [&](int g, int s, float2 x, float2 y) {
+      const float f = w[s];
+      a[g].x = fmaf(f, x.x, a[g].x);
+      a[g].y = fmaf(f, x.y, a[g].y);
+      b[g].x = fmaf(f, y.x, b[g].x);
+      b[g].y = fmaf(f, y.y, b[g].y);
+    };
+    auto load = [&](int s, int col) {
+      return col < cols ? src[static_cast<int64_t>(s) * cols + col] : make_float2(0.f, 0.f);
+    };
+    int s0 = W == 1 ? 0 : warp;
+    if (W == 4 && c0 == 0) {
 #pragma unroll
-      for (int g = 0; g < SUMS; ++g) {
-        const int s = s0 + g;
-        if (s < used) {
-          const float f = w[s];
-          if (c < cols) {
-            const float2 x = src[static_cast<int64_t>(s) * cols + c];
-            a[g].x = fmaf(f, x.x, a[g].x);
-            a[g].y = fmaf(f, x.y, a[g].y);
-          }
-          if (d < cols) {
-            const float2 y = src[static_cast<int64_t>(s) * cols + d];
-            b[g].x = fmaf(f, y.x, b[g].x);
-            b[g].y = fmaf(f, y.y, b[g].y);
-          }
-        }
-      }
+      for (int i = 0; i < EARLY; ++i, s0 += 4)
+        if (s0 < used) add(0, s0, early[i][0], early[i][1]);
+    }
+#pragma unroll(W == 1 ? 2 : 8)
+    for (; s0 < used; s0 += 4) {
+#pragma unroll
+      for (int g = 0; g < SUMS; ++g)
+        if (s0 + g < used) add(g, s0 + g, load(s0 + g, c), load(s0 + g, d));
     }
     if constexpr (W == 1) {
       a[0].x = (a[0].x + a[1].x) + (a[2].x + a[3].x);
