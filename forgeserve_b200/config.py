@@ -11,6 +11,8 @@ _SCALING_KEYS = {"linear": {"factor"}, "ntk": {"factor"},
 def check_rope_scaling(scaling: Optional[dict]) -> None:
     if scaling is None:
         return
+    if not isinstance(scaling, dict):
+        raise ValueError("rope_scaling must be a dict with a kind and a factor")
     kind = scaling.get("kind")
     if kind not in _SCALING_KEYS:
         raise ValueError(f"rope_scaling kind must be one of {sorted(_SCALING_KEYS)}, not {kind!r}")

@@ -765,11 +765,11 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int h = warp * 8 * NT + 8 * n + 2 * tl + c;
-      const float f = exp2f(mo[n][c] - m[n][c]);
+      const float f = exp2f(0.5f * (mo[n][c] - m[n][c]));   // twice: scales near fp32's end leave its range at once
 #pragma unroll
       for (int i = 0; i < G::KS; ++i)
         *reinterpret_cast<float2*>(osm + h * G::O_ROW + i / (G::VB / 2) * 128 + gl * G::VB + 2 * (i % (G::VB / 2))) =
-            make_float2(acc[n][i][c] * f, acc[n][i][c + 2] * f);
+            make_float2(acc[n][i][c] * f * f, acc[n][i][c + 2] * f * f);
       if (gl == 0) {
         msm[2 * h] = m[n][c];
         msm[2 * h + 1] = l[n][c];

@@ -424,7 +424,8 @@ int write_t(const WriteParams& p, bool quant, int interleaved, cudaStream_t st) 
   constexpr int PIECES = 32 / static_cast<int>(sizeof(T));   // values a lane of the vector form holds of a head
   int lanes = 1;
   while (lanes * PIECES < p.hd) lanes *= 2;
-  if (write_vec_ok<T>(p, quant, interleaved)) {
+  const int64_t vec_items = p.tokens * ((p.nh + 2 * p.nkv + 1) / 2) * lanes;   // thread numbers of 31 bits (two heads each)
+  if (write_vec_ok<T>(p, quant, interleaved) && vec_items <= INT32_MAX) {
     // bf16: two heads a thread and one wave of CTAs that stay (8192 tokens of 32 + 8 + 8 heads into the 8-bit cache: 35 us,
     // 41 with a CTA for every 256 threads of work; four heads 40, 88 % of HBM to the bf16 cache). fp32 moves twice the
     // bytes with half the arithmetic: four heads and four waves (58 us, 94 %; one wave 64).
@@ -433,7 +434,6 @@ int write_t(const WriteParams& p, bool quant, int interleaved, cudaStream_t st) 
     const int64_t vec_blocks = (p.tokens * groups * lanes + 255) / 256;
     auto kernel = quant ? (interleaved ? rotary_write_vec_kernel<T, true, true, HEADS> : rotary_write_vec_kernel<T, true, false, HEADS>)
                         : (interleaved ? rotary_write_vec_kernel<T, false, true, HEADS> : rotary_write_vec_kernel<T, false, false, HEADS>);
-    if (vec_blocks >= 1 << 24) return fail("rotary_kv_write: too many tokens");   // 32-bit thread numbers
     const int64_t ctas = 148 * 4 * (sizeof(T) == 4 ? 4 : 1);
     launch_pdl_async(kernel, static_cast<unsigned>(vec_blocks < ctas ? vec_blocks : ctas), 256, 0, st, p, lanes, groups);
     return check_launch("rotary_write_vec_kernel");

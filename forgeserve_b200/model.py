@@ -86,7 +86,7 @@ class RopeTables:
     """fp32 cos/sin tables per device; the kernels round them to the activation dtype as the reference does."""
 
     def __init__(self, cfg: ModelConfig):
-        if cfg.rope_scaling is None and cfg.rotary_width == cfg.head_dim:
+        if cfg.rope_scaling is None and cfg.rope_layout == "half" and cfg.rotary_width == cfg.head_dim:
             self.cos, self.sin = precompute_rope(cfg.head_dim, cfg.max_seq_len, cfg.rope_theta)
         else:
             self.cos, self.sin = rope_tables(cfg.rotary_width, cfg.max_seq_len, cfg.rope_theta, cfg.rope_scaling)

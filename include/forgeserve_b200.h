@@ -175,7 +175,7 @@ int fs_attention_decode_static(const void* q, int64_t ldq, const fs_kv_cache* kv
  *
  * fs_kv_quant: a cache of e4m3 codes. `cache` addresses the codes as fs_kv_cache addresses values (k and v point to
  * bytes); slot s of row r, KV head g has its scales at table[...] * scale_block_stride + g * scale_head_stride +
- * s % block_size of k_scale and v_scale. A value is code * scale. */
+ * s % block_size of k_scale and v_scale. A value is code * scale; scales are not negative. */
 typedef struct {
   fs_kv_cache cache;
   float* k_scale;

@@ -427,6 +427,8 @@ def test_decode_special_values(dtype, hd):
     ks[table[2]] *= 1e-30
     q[2] = (q[2].double() * 1e30).to(dtype)
     ks[table[3]] *= 30.0                                            # scores of several hundred: one key takes it all
+    vs[table[3]] *= 2.0 ** 123                                      # values near fp32's end
+    v.view(torch.uint8)[table[3]] &= 0x8F                           # (their codes below 0.02, so that none leaves it)
     vs[table[4]] *= 1e-38
     q[5] = 0.0
     out = check_decode(q, pools, table, positions, n_slots, nh, nkv, hd)
@@ -574,6 +576,40 @@ def test_two_captured_graphs_and_another_stream():
         torch.cuda.synchronize()
         for (o, (kd, vd)), (wo, wk, wv) in zip(outs, want):
             assert torch.equal(o, wo) and torch.equal(kd, wk) and torch.equal(vd, wv)
+
+
+def test_a_side_stream_and_two_threads():
+    """The chain on a stream of its own, and from two host threads at once on two streams, gives the default stream's
+    bits."""
+    import threading
+
+    nh, nkv, hd, bs = 8, 2, 64, 16
+    cos, sin = (t.to(DEV) for t in rope_tables(hd, 4096, 10000.0))
+    sets, want = [], []
+    for seed in (3, 4):
+        q, pools, table, positions, n_slots = decode_case(torch.bfloat16, [1500, 700], nh, nkv, hd, bs, seed=seed)
+        qkv = torch.randn(2, (nh + 2 * nkv) * hd, generator=gen(seed), device=DEV).bfloat16()
+        sets.append((pools, table, qkv, cos, sin, positions, n_slots, nh, nkv, hd))
+        out, (kd, vd) = chain(*sets[-1])
+        want.append((out, kd, vd))
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(30):
+                out, (kd, vd) = chain(*sets[i])
+            got[i] = (out, kd, vd)
+        st.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
 
 
 FIRST_CALL_CAPTURED = """

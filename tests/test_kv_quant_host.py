@@ -29,7 +29,7 @@ def test_config_rotary_fields():
     cfg = ModelConfig(rope_layout="interleaved", rotary_dim=8, rope_scaling={"kind": "linear", "factor": 2.0})
     assert ModelConfig(**cfg.to_dict()) == cfg and cfg.rotary_width == 8
     for bad in (dict(rope_layout="both"), dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=18),
-                dict(rope_scaling={"kind": "other", "factor": 2}), dict(rope_scaling={"kind": "linear"}),
+                dict(rope_scaling={"kind": "other", "factor": 2}), dict(rope_scaling="linear"), dict(rope_scaling={"kind": "linear"}),
                 dict(rope_scaling={"kind": "linear", "factor": 0.5}),
                 dict(rope_scaling={"kind": "linear", "factor": 2, "beta_fast": 1}),
                 dict(rope_scaling={"kind": "by_parts", "factor": 2}),
