@@ -294,17 +294,18 @@ struct Geo {
   static constexpr int BOX = HD < 128 ? 64 : 128;             // bytes of a box's row
   static constexpr int BOXES = HD / BOX;                      // boxes a row
   static constexpr int STEP_BYTES = STEP * HD;                // K (or V) of a step
-  // One step deep: K of the next step is on its way from the scores on, its V from the V product on. Two steps take the
-  // shared memory of a fourth CTA an SM (64 rows: 89 us against 80).
-  static constexpr int STAGES = 1;
-  static constexpr int BUF = 2 * STAGES * STEP_BYTES;         // a warp's ring: K stages, then V stages
+  // A warp's ring is one step deep: K of the next step is on its way from the scores on, its V from the V product on. Two
+  // steps take the shared memory of a fourth CTA an SM (64 rows: 89 us against 80), four for CTAs alone on an SM save 0.3
+  // us of 11.
+  static constexpr int BUF = 2 * STEP_BYTES;                  // a warp's K, then V
   static constexpr int Q_OFF = WARPS * BUF;                   // q as B operands: [NT][PARTS][KS][32 lanes] of 8 bytes
   static constexpr int AT_OFF = Q_OFF + NT * PARTS * KS * 256;   // where tiles or keys lie: [2][values, scales][WARPS][LOOK]
   static constexpr int LOOK = SEG * (WHOLE ? 2 : STEP);
-  static constexpr int BAR_OFF = AT_OFF + 2 * WARPS * LOOK * 16;   // a warp's barriers: K stages, V stages
-  static constexpr int END = BAR_OFF + (WHOLE ? WARPS * 2 * STAGES * 8 : 0);
+  static constexpr int BAR_OFF = AT_OFF + 2 * WARPS * LOOK * 16;   // a warp's barriers, K and V: past what the merge uses
+  static constexpr int END = BAR_OFF + (WHOLE ? WARPS * 16 : 0);
   static constexpr int O_ROW = HD + 4;                        // padded: the lanes' writes spread over the banks
   static constexpr int O_BYTES = WARPS * 8 * NT * (O_ROW + 3) * 4;   // the warps' sums, (max, sum), weights, over all that
+  static_assert(!WHOLE || O_BYTES <= BAR_OFF, "the merge must leave the barriers alone");
   static constexpr int SMEM = (O_BYTES > END ? O_BYTES : END) + (WHOLE ? 1024 : 0);   // boxes lie on 1024 bytes
   // CTAs an SM that the registers are held to: the most that spill little (hd 128: 80 us on 64 rows at 4, 87 at 3; 16 heads
   // a KV head 65 at 3, 76 unbounded; hd 64, MHA 50 at 6, 55 at 4; hd 256 31 at 3, 34 unbounded).
@@ -324,38 +325,22 @@ __device__ __forceinline__ int k_chunk(int t, int c) {
   return HD == 64 ? t : WHOLE ? (c >> 1) * 8 + 2 * t + (c & 1) : 4 * c + t;
 }
 
+struct Row {   // what a CTA works on: a row's query heads h0 .. h0 + heads - 1 of one KV head
+  int64_t r, n_vis, per;
+  int kvh, h0, heads;
+};
+
+// One split of a row. phase: steps that this warp's barriers have seen. False if a copy did not come in time.
 template <typename T, int HD, int NT, bool WHOLE>
-__global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
-    quant_decode_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Params p) {
-  pdl_trigger();
+__device__ __forceinline__ bool decode_split(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, uint8_t* smem,
+                                             const Row& row, int split, uint32_t phase) {
   using G = Geo<T, HD, NT, WHOLE>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = WHOLE ? reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023))
-                        : smem_raw;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, tl = lane & 3;
+  const int64_t r = row.r, n_vis = row.n_vis, per = row.per, begin = split * per;
+  const int kvh = row.kvh, h0 = row.h0, heads = row.heads;
   uint8_t* buf = smem + warp * G::BUF;
-  uint64_t* kbar = reinterpret_cast<uint64_t*>(smem + G::BAR_OFF) + warp * 2 * G::STAGES;
-  uint64_t* vbar = kbar + G::STAGES;
-  if constexpr (WHOLE) {
-    if (lane == 0) {
-      for (int i = 0; i < 2 * G::STAGES; ++i) mbar_init(&kbar[i], 1);
-      fence_barrier_init();
-      prefetch_tmap(&tmK);
-      prefetch_tmap(&tmV);
-    }
-    __syncwarp();
-  }
-  pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
-  const int split = blockIdx.x, kvh = blockIdx.y / p.groups, h0 = (blockIdx.y % p.groups) * 8 * NT;
-  const int64_t r = blockIdx.z;
-  const int heads = p.rep - h0 < 8 * NT ? p.rep - h0 : 8 * NT;
-  const int64_t n_vis = visible(p, r), per = split_keys(n_vis, p.nkv), begin = split * per;
-  if (begin >= n_vis) {
-    if (p.splits == 1)   // a row that sees nothing
-      for (int i = threadIdx.x; i < heads * p.hd; i += blockDim.x)
-        static_cast<T*>(p.out)[r * p.ldo + static_cast<int64_t>(kvh * p.rep + h0) * p.hd + i] = from_f<T>(0.f);
-    return;              // the join does not read an empty split
-  }
+  uint64_t* kbar = reinterpret_cast<uint64_t*>(smem + G::BAR_OFF) + warp * 2;
+  uint64_t* vbar = kbar + 1;
   const int n_keys = static_cast<int>(n_vis - begin < per ? n_vis - begin : per);
   const int n_steps = (n_keys + STEP - 1) / STEP;
   const int my_n = n_steps > warp ? (n_steps - warp + WARPS - 1) / WARPS : 0;   // steps warp, warp + WARPS, ..
@@ -413,7 +398,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
   auto issue_k = [&](int j) {
     const int64_t* a = place(j);
     if constexpr (WHOLE) {
-      load_boxes(&tmK, buf + (j % G::STAGES) * G::STEP_BYTES, &kbar[j % G::STAGES], a);
+      load_boxes(tmK, buf, kbar, a);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -431,7 +416,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
   auto issue_v = [&](int j) {
     const int64_t* a = place(j);
     if constexpr (WHOLE) {
-      load_boxes(&tmV, buf + (G::STAGES + j % G::STAGES) * G::STEP_BYTES, &vbar[j % G::STAGES], a);
+      load_boxes(tmV, buf + G::STEP_BYTES, vbar, a);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -459,9 +444,9 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
     if constexpr (!WHOLE) asm volatile("cp.async.commit_group;" ::: "memory");
   };
   // Waits for K (V) of step j; false if it did not come within the time limit.
-  auto wait = [&](uint64_t* bars, int j) -> bool {
+  auto wait = [&](uint64_t* bar, int j) -> bool {
     if constexpr (WHOLE) {
-      return __all_sync(0xffffffffu, mbar_wait(&bars[j % G::STAGES], static_cast<uint32_t>((j / G::STAGES) & 1), p.err));
+      return __all_sync(0xffffffffu, mbar_wait(bar, (phase + j) & 1, p.err));
     } else {
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       return true;
@@ -469,13 +454,10 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
   };
   look_up(0);
   if (my_n > 0) load_scales(0);
-#pragma unroll
-  for (int j = 0; j < G::STAGES; ++j) {
-    if (j < my_n) issue_k(j);
-    commit();
-    if (j < my_n) issue_v(j);
-    commit();
-  }
+  if (my_n > 0) issue_k(0);
+  commit();
+  if (my_n > 0) issue_v(0);
+  commit();
 
   // Q as B operands: lane (gl, tl) holds of head 8 n + gl the dims 16 k_chunk(tl, c) + 4 i + 0..3, k step 4 c + i, after
   // the head's scale. Every warp finds the scales, and writes its share of the k steps to shared memory.
@@ -558,8 +540,6 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
       late = 1;
       break;
     }
-    const uint8_t* kbuf = buf + (j % G::STAGES) * G::STEP_BYTES;
-    const uint8_t* vbuf = buf + (G::STAGES + j % G::STAGES) * G::STEP_BYTES;
     float s[2][NT][4];   // keys 16 t + gl (c 0, 1) and + 8 (c 2, 3)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -572,8 +552,8 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
       for (int c = 0; c < G::KC; ++c) {
         const int a0_at = WHOLE ? G::box_at(t * TILE + gl, k_chunk<HD, WHOLE>(tl, c)) : ((2 * t * G::KC + c) * 32 + lane) * 16;
         const int a1_at = WHOLE ? G::box_at(t * TILE + gl + 8, k_chunk<HD, WHOLE>(tl, c)) : a0_at + G::KC * 512;
-        const uint4 u = *reinterpret_cast<const uint4*>(kbuf + a0_at);
-        const uint4 w = *reinterpret_cast<const uint4*>(kbuf + a1_at);
+        const uint4 u = *reinterpret_cast<const uint4*>(buf + a0_at);
+        const uint4 w = *reinterpret_cast<const uint4*>(buf + a1_at);
         const uint32_t ku[4] = {u.x, u.y, u.z, u.w}, kw[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -596,7 +576,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
         }
     }
     __syncwarp();
-    if (j + G::STAGES < my_n) issue_k(j + G::STAGES);   // over the K just read
+    if (j + 1 < my_n) issue_k(j + 1);   // over the K just read
     commit();
 
     // Scores in the log2 domain; e: the exponent (fp32: its whole part) of the value's scale.
@@ -694,7 +674,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
     if (WHOLE && left < STEP) {   // whatever lies behind the last visible key, NaN codes too, becomes zeros
       for (int i = lane; i < (STEP - left) * (HD / 16); i += 32) {
         const int row = left + i / (HD / 16);
-        *reinterpret_cast<uint4*>(buf + (G::STAGES + j % G::STAGES) * G::STEP_BYTES + G::box_at(row, i % (HD / 16))) =
+        *reinterpret_cast<uint4*>(buf + G::STEP_BYTES + G::box_at(row, i % (HD / 16))) =
             make_uint4(0, 0, 0, 0);
       }
       __syncwarp();
@@ -710,7 +690,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
           const int row = t * TILE + 2 * tl + (i & 1) + 4 * (i & 2);
           const int v_at = !WHOLE ? (((t * 4 + i) * G::VC + c) * 32 + lane) * G::VB
                                   : HD == 64 ? G::box_at(row, gl >> 1) + (gl & 1) * 8 : G::box_at(row, c * 8 + gl);
-          const uint8_t* src = vbuf + v_at;
+          const uint8_t* src = buf + G::STEP_BYTES + v_at;
           if constexpr (G::VB == 16) {
             const uint4 u = *reinterpret_cast<const uint4*>(src);
             v[i][0] = u.x, v[i][1] = u.y, v[i][2] = u.z, v[i][3] = u.w;
@@ -734,16 +714,14 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
           }
       }
     __syncwarp();
-    if (j + G::STAGES < my_n) issue_v(j + G::STAGES);
+    if (j + 1 < my_n) issue_v(j + 1);
     commit();
   }
   if constexpr (WHOLE) {
     if (late) {   // let the copies in flight land (bounded) before the shared memory is given back or used again
-      const int k0 = late == 1 ? j : j + 1;   // K of step j is in use already where V did not come
-      for (int k = k0; k < k0 + G::STAGES && k < my_n; ++k)
-        mbar_wait(&kbar[k % G::STAGES], static_cast<uint32_t>((k / G::STAGES) & 1), p.err);
-      for (int k = j; k < j + G::STAGES && k < my_n; ++k)
-        mbar_wait(&vbar[k % G::STAGES], static_cast<uint32_t>((k / G::STAGES) & 1), p.err);
+      const int k = late == 1 ? j : j + 1;   // the K in flight
+      if (k < my_n) mbar_wait(kbar, (phase + k) & 1, p.err);
+      mbar_wait(vbar, (phase + j) & 1, p.err);
     }
   } else {
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -756,7 +734,7 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], o);
-  if (__syncthreads_or(late)) return;   // buffers, q and offsets are free; a CTA that gave up leaves no result
+  if (__syncthreads_or(late)) return false;   // buffers, q and offsets are free; a CTA that gave up leaves no result
   float* osm = reinterpret_cast<float*>(smem);                     // [WARPS][8 NT][O_ROW]
   float* msm = osm + WARPS * 8 * NT * G::O_ROW;                    // [WARPS][8 NT][2]
   float* wsm = msm + WARPS * 8 * NT * 2;                           // [8 NT][WARPS]
@@ -819,6 +797,53 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
       *reinterpret_cast<float4*>(p.ws + (part0 + static_cast<int64_t>(h) * p.splits) * p.hd + d) = o;
     }
   }
+  return true;
+}
+
+template <typename T, int HD, int NT, bool WHOLE>
+__global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
+    quant_decode_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Params p) {
+  pdl_trigger();
+  pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
+  using G = Geo<T, HD, NT, WHOLE>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = WHOLE ? reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023))
+                        : smem_raw;
+  Row row;
+  row.r = blockIdx.z;
+  row.kvh = blockIdx.y / p.groups;
+  row.h0 = (blockIdx.y % p.groups) * 8 * NT;
+  row.heads = p.rep - row.h0 < 8 * NT ? p.rep - row.h0 : 8 * NT;
+  row.n_vis = visible(p, row.r);
+  row.per = split_keys(row.n_vis, p.nkv);
+  if (blockIdx.x * row.per >= row.n_vis) {   // the join does not read an empty split
+    if (p.splits == 1)                       // a row that sees nothing
+      for (int i = threadIdx.x; i < row.heads * p.hd; i += blockDim.x)
+        static_cast<T*>(p.out)[row.r * p.ldo + static_cast<int64_t>(row.kvh * p.rep + row.h0) * p.hd + i] = from_f<T>(0.f);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if constexpr (WHOLE) {
+    if (lane == 0) {
+      uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::BAR_OFF) + warp * 2;
+      mbar_init(&bars[0], 1);
+      mbar_init(&bars[1], 1);
+      fence_barrier_init();
+    }
+    __syncwarp();
+  }
+  // A grid that would hold many CTAs for splits that no row has (a table much wider than its rows) takes them in turn.
+  uint32_t phase = 0;
+  for (int split = blockIdx.x; split * row.per < row.n_vis; split += gridDim.x) {
+    if (split != static_cast<int>(blockIdx.x)) {
+      fence_proxy_async_smem();   // the merge's shared memory is the next split's ring
+      __syncthreads();
+    }
+    if (!decode_split<T, HD, NT, WHOLE>(p, &tmK, &tmV, smem, row, split, phase)) return;
+    const int64_t left = row.n_vis - split * row.per, keys = left < row.per ? left : row.per;
+    const int steps = static_cast<int>((keys + STEP - 1) / STEP);
+    phase += steps > warp ? (steps - warp + WARPS - 1) / WARPS : 0;
+  }
 }
 
 bool supported(const Params& p) {
@@ -856,7 +881,10 @@ int launch_geo(Params p, int64_t B, int64_t nkv, cudaStream_t st) {
       return check_launch("quant_decode_tc set smem");
     attr[dev] = true;
   }
-  const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(nkv * p.groups), static_cast<unsigned>(B));
+  // at most 8 waves of CTAs: in a wider grid most stand for splits that no row has
+  const int64_t each = (8 * ONE_WAVE + nkv * p.groups * B - 1) / (nkv * p.groups * B);
+  const dim3 grid(static_cast<unsigned>(p.splits < each ? p.splits : each), static_cast<unsigned>(nkv * p.groups),
+                  static_cast<unsigned>(B));
   launch_pdl_async(quant_decode_tc_kernel<T, HD, NT, WHOLE>, grid, 32 * WARPS, G::SMEM, st, mk, mv, p);
   return check_launch("quant_decode_tc_kernel");
 }

@@ -514,6 +514,25 @@ def test_decode_bits_do_not_depend_on_the_batch(dtype, nh, nkv, hd, bs):
         assert torch.equal(one[0], whole[r])
 
 
+@pytest.mark.parametrize("dtype,bs", [(torch.bfloat16, 16), (torch.bfloat16, 20), (torch.float32, 48)])
+def test_decode_takes_several_splits_in_turn(dtype, bs):
+    """A batch with more splits than CTAs are launched for: each row as it comes alone, one row against 64 bits."""
+    nh, nkv, hd, B = 32, 32, 64, 48
+    lengths = [1 + (i * 1237) % 5000 for i in range(B)]
+    lengths[5] = 0
+    q, pools, table, positions, n_slots = decode_case(dtype, lengths, nh, nkv, hd, bs, seed=12)
+    whole = torch.empty_like(q)
+    ops.attention_decode_quant(q, ops.quant_paged_desc(*pools, table), n_slots, positions, whole, B, nh, nkv, hd)
+    assert not whole[5].any()
+    for r in (0, 5, 11, 23, 47, max(range(B), key=lambda i: lengths[i])):
+        one = torch.empty_like(q[:1])
+        ops.attention_decode_quant(q[r: r + 1], ops.quant_paged_desc(*pools, table[r: r + 1]), n_slots,
+                                   positions[r: r + 1], one, 1, nh, nkv, hd)
+        assert torch.equal(one[0], whole[r])
+    r = max(range(B), key=lambda i: lengths[i])
+    check_decode(q[r: r + 1], pools, table[r: r + 1], positions[r: r + 1], n_slots, nh, nkv, hd)
+
+
 def test_pool_slices_and_strided_rows():
     """Heads of a larger pool, rows of q and out inside wider tensors, a table cut from a wider one."""
     nkv, hd, bs, nh = 2, 128, 16, 8
