@@ -224,7 +224,8 @@ __global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p,
   const int c = threadIdx.x & (lanes - 1), heads = p.nh + 2 * p.nkv, half = p.rd / 2;
   const unsigned per = 256u / lanes, items = static_cast<unsigned>(p.tokens) * groups;
   // Where the pieces of q and k heads lie, and of v heads.
-  const bool turns = IL || c * 2 * VEC < p.rd;   // IL: pair by pair below
+  const bool turns = IL || c * 2 * VEC < p.rd;       // IL: pair by pair below,
+  const bool all_turn = !IL || p.rd == p.hd;         // unless all do
   int lo = VEC * c, hi = p.hd / 2 + VEC * c;
   const int lo_v = lo, hi_v = hi;
   if (!IL) {
@@ -292,13 +293,13 @@ __global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p,
       float x[2 * VEC];
       unpack_piece(raw[u][0], x, static_cast<const T*>(nullptr));
       unpack_piece(raw[u][1], x + VEC, static_cast<const T*>(nullptr));
-      if (!v) {
+      if (!v && turns) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          if (pair_of(i) < half) {
-            float& a = x[IL ? 2 * i : i];
-            float& b = x[IL ? 2 * i + 1 : VEC + i];
-            const float a0 = a, b0 = b;
+          float& a = x[IL ? 2 * i : i];
+          float& b = x[IL ? 2 * i + 1 : VEC + i];
+          const float a0 = a, b0 = b;
+          if (!IL || all_turn || pair_of(i) < half) {
             a = a0 * cs[i] - b0 * sn[i];
             b = b0 * cs[i] + a0 * sn[i];
           }
