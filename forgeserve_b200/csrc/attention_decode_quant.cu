@@ -6,7 +6,7 @@
 // so a scale is one factor on a score or on a probability, and the products run on the codes themselves.
 // The floor is the cache's bytes: 2 (hd + 4) for each visible slot of each KV head, read once for all its query heads.
 //
-// A row's slots are cut into splits, one CTA each; quant_combine_kernel joins them. How they are cut follows from the
+// A row's slots are cut into splits, a CTA's work each; quant_combine_kernel joins them. How they are cut follows from the
 // row's visible slots and the KV heads alone (split_keys), so the order of a row's sums does not depend on the batch or
 // on the table's width (a step gives the same bits eagerly, in a CUDA graph with a padded table, or in micro-batches).
 // Workspace (fp32): sums [B][nh][splits][hd], then (max, sum) [B][nh][splits][2] in the log2 domain.
@@ -906,9 +906,9 @@ int launch_t(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
 }  // namespace tc
 
 // Joins the splits of a (row, head), W warps (1 or 4) each: weights exp2(m_split - m), then four interleaved sums over the
-// splits, joined pairwise; the order, and so the bits, are the same for both W. One warp each where there are many
-// (row, head) pairs (64 rows x 32 heads of 9 splits: 2 us less than a CTA each), four where there are few and a
-// warp's loads would come one after another (1 row x 32 heads of 8 splits: 1.4 us less).
+// splits, joined pairwise; the order, and so the bits, are the same for both W. Four warps each while their CTAs are few,
+// the loads then come at once (1024 pairs of 4 splits of hd 256: 28 us with the splits against 31); one warp each from
+// 4096 pairs on (4096 pairs of 8 splits of hd 128: 63 us against 67).
 constexpr int MAX_SPLITS = ONE_WAVE;
 template <typename T, int W>
 __global__ void __launch_bounds__(128) quant_combine_kernel(Params p) {
@@ -1035,7 +1035,7 @@ int launch_t(const Params& p, int64_t B, int64_t nkv, cudaStream_t st) {
   if (tc::supported(p) ? tc::launch_t<T>(p, B, nkv, st) : launch_any<T>(p, B, nkv, st)) return -1;
   if (p.splits == 1) return 0;
   const int64_t pairs = B * p.nh;
-  if (pairs >= 1024)
+  if (pairs >= 4096)
     launch_pdl_async(quant_combine_kernel<T, 1>, static_cast<unsigned>((pairs + 3) / 4), 128, 0, st, p);
   else
     launch_pdl_async(quant_combine_kernel<T, 4>, static_cast<unsigned>(pairs), 128, 0, st, p);

@@ -496,7 +496,8 @@ def test_decode_is_independent_of_batch_and_table_width():
 
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd,bs", [(torch.bfloat16, 32, 4, 128, 16), (torch.float32, 32, 16, 64, 16),
-                                                (torch.bfloat16, 32, 8, 128, 20), (torch.bfloat16, 32, 8, 40, 16)])
+                                                (torch.bfloat16, 32, 8, 128, 20), (torch.bfloat16, 32, 8, 40, 16),
+                                                (torch.bfloat16, 128, 8, 128, 16)])
 def test_decode_bits_do_not_depend_on_the_batch(dtype, nh, nkv, hd, bs):
     """Rows of a batch large enough for another join, and behind a table of other width, against each row alone."""
     lengths = [1 + (i * 797) % 3000 for i in range(40)]
