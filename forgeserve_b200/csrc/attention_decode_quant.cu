@@ -6,9 +6,9 @@
 // so a scale is one factor on a score or on a probability, and the products run on the codes themselves.
 // The floor is the cache's bytes: 2 (hd + 4) for each visible slot of each KV head, read once for all its query heads.
 //
-// A row's slots are cut into splits, a CTA's work each; quant_combine_kernel joins them. How they are cut follows from the
-// row's visible slots and the KV heads alone (split_keys), so the order of a row's sums does not depend on the batch or
-// on the table's width (a step gives the same bits eagerly, in a CUDA graph with a padded table, or in micro-batches).
+// A row's slots are cut into splits, a CTA's work each; quant_combine_kernel joins them. How they are cut follows from
+// the row's visible slots and the KV heads alone (split_keys), so the order of a row's sums does not depend on the batch
+// or on the table's width (a step gives the same bits eagerly, in a CUDA graph with a padded table, or in micro-batches).
 // Workspace (fp32): sums [B][nh][splits][hd], then (max, sum) [B][nh][splits][2] in the log2 domain.
 //
 // A row with a negative position sees nothing and gets zeros. A block number outside the cache reads as zero rows and
@@ -64,8 +64,9 @@ __device__ __forceinline__ int64_t visible(const Params& p, int64_t r) {
 // max that an exponent may be taken against: -infinity (no finite score) becomes 0, so that exp2(-inf - m) is 0.
 __device__ __forceinline__ float safe_max(float m) { return m == -INFINITY ? 0.f : m; }
 
-// What the tensor-core kernel below does not take (hd no multiple of 16, rows off 16 bytes): any hd <= 256 and layout, 32 keys at a time as fp32 in shared memory; a warp owns two query heads, a lane
-// one key of the scores and hd / 32 dims of the sums.
+// What the tensor-core kernel below does not take (hd no multiple of 16, rows off 16 bytes): any hd <= 256 and layout, 32
+// keys at a time as fp32 in shared memory; a warp owns two query heads, a lane one key of the scores and hd / 32 dims of
+// the sums.
 template <typename T>
 __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
   pdl_trigger();
@@ -171,9 +172,10 @@ __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
 }
 
 // ------------------------------------------------------------------------------------ tensor-core kernel
-// hd a multiple of 16 up to 256, 16-byte rows; the kernel is built for HD = 64, 128 and 256, dims from hd on are zeros in
-// shared memory (no bytes of the cache). The codes are exact in f16, so both products run as mma.sync m16n8k16 f16 with fp32
-// sums and the scales never touch them; the query heads of the KV head are the N side (NT tiles of 8):
+// hd a multiple of 16 up to 256, 16-byte rows; the kernel is built for HD = 64, 128 and 256, dims from hd on are zeros
+// in shared memory (no bytes of the cache). The codes are exact in f16, so both products run as mma.sync m16n8k16 f16
+// with fp32 sums and the scales never touch them; the query heads of the KV head are the N side (NT tiles of 8). A tcgen05
+// product would want the codes widened in shared memory first; here they are widened in registers:
 //     S^T (16 keys x 8 heads) = K (16 x hd) Q^T (hd x 8),   O^T (hd x 8 heads) += V^T (hd x 16) P^T (16 x 8)
 // A contraction's index order is free as long as both operands agree, and so are the rows of O^T; they are chosen so
 // that every lane's operand values are neighbouring bytes of a cache row: lane (g, t) = (lane / 4, lane % 4) takes, of
@@ -181,8 +183,8 @@ __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
 // g for V (8 bytes of it at hd 64). P^T reaches the B layout by movmatrix.
 //
 // A warp takes STEP keys at a time, into a ring of its own; no barrier joins the warps before the end.
-//   WHOLE (the block size is a multiple of 16, so a tile of 16 keys lies in one block): TMA boxes of 16 rows, swizzled over
-//     128 (hd 64: 64) bytes, under which both fragment reads above are free of bank conflicts.
+//   WHOLE (the block size is a multiple of 16, so a tile of 16 keys lies in one block): TMA boxes of 16 rows, swizzled
+//     over 128 (hd 64: 64) bytes, under which both fragment reads above are free of bank conflicts.
 //   otherwise every key is looked up by itself and each lane copies exactly the bytes it will use (cp.async).
 //
 // Q enters as f16 after a scale by a power of two that brings each head's largest |q| to [1, 2): exact for bf16 down to
@@ -191,6 +193,9 @@ __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
 // widely keep the f16 range: P = exp2(s + log2 vs - mo), mo >= max(s + log2 vs) - SLACK. fp32 takes log2 vs as exponent
 // and mantissa, and P's remainder as a second product. Maxima are raised only when a score exceeds them by SLACK: one
 // vote a step instead of a reduction.
+//
+// 64 rows of 2176 to 4352 slots of 8 x 128 values, 32 query heads: 78 us with the join, 86 % of HBM (bf16 queries); 2
+// rows of 131072: 91 us, 92 %. The copies alone, without a product, take 68 us of the first, the join 6.
 namespace tc {
 
 constexpr int WARPS = 4, TILE = 16, STEP = 32;   // a warp takes STEP keys (two tiles) at a time
@@ -294,21 +299,21 @@ struct Geo {
   static constexpr int BOX = HD < 128 ? 64 : 128;             // bytes of a box's row
   static constexpr int BOXES = HD / BOX;                      // boxes a row
   static constexpr int STEP_BYTES = STEP * HD;                // K (or V) of a step
-  // A warp's ring is one step deep: K of the next step is on its way from the scores on, its V from the V product on. Two
-  // steps take the shared memory of a fourth CTA an SM (64 rows: 89 us against 80), four for CTAs alone on an SM save 0.3
-  // us of 11.
+  // A warp's ring is one step deep: K of the next step is on its way from the scores on, its V from the V product on.
+  // Two steps take the shared memory of a fourth CTA an SM (64 rows: 89 us against 80), four for CTAs alone on an SM save
+  // 0.3 us of 11.
   static constexpr int BUF = 2 * STEP_BYTES;                  // a warp's K, then V
   static constexpr int Q_OFF = WARPS * BUF;                   // q as B operands: [NT][PARTS][KS][32 lanes] of 8 bytes
-  static constexpr int AT_OFF = Q_OFF + NT * PARTS * KS * 256;   // where tiles or keys lie: [2][values, scales][WARPS][LOOK]
+  static constexpr int AT_OFF = Q_OFF + NT * PARTS * KS * 256;   // places: [2][values, scales][WARPS][LOOK]
   static constexpr int LOOK = SEG * (WHOLE ? 2 : STEP);
-  static constexpr int BAR_OFF = AT_OFF + 2 * WARPS * LOOK * 16;   // a warp's barriers, K and V: past what the merge uses
+  static constexpr int BAR_OFF = AT_OFF + 2 * WARPS * LOOK * 16;   // a warp's barriers, K and V
   static constexpr int END = BAR_OFF + (WHOLE ? WARPS * 16 : 0);
   static constexpr int O_ROW = HD + 4;                        // padded: the lanes' writes spread over the banks
-  static constexpr int O_BYTES = WARPS * 8 * NT * (O_ROW + 3) * 4;   // the warps' sums, (max, sum), weights, over all that
+  static constexpr int O_BYTES = WARPS * 8 * NT * (O_ROW + 3) * 4;   // the merge: sums, (max, sum), weights
   static_assert(!WHOLE || O_BYTES <= BAR_OFF, "the merge must leave the barriers alone");
   static constexpr int SMEM = (O_BYTES > END ? O_BYTES : END) + (WHOLE ? 1024 : 0);   // boxes lie on 1024 bytes
-  // CTAs an SM that the registers are held to: the most that spill little (hd 128: 80 us on 64 rows at 4, 87 at 3; 16 heads
-  // a KV head 65 at 3, 76 unbounded; hd 64, MHA 50 at 6, 55 at 4; hd 256 31 at 3, 34 unbounded).
+  // CTAs an SM that the registers are held to: the most that spill little (hd 128: 80 us on 64 rows at 4, 87 at 3; 16
+  // heads a KV head 65 at 3, 76 unbounded; hd 64, MHA 50 at 6, 55 at 4; hd 256 31 at 3, 34 unbounded).
   static constexpr int CTAS = NT == 1 ? (HD == 64 ? (sizeof(T) == 2 ? 6 : 5) : HD == 128 ? 4 : 3)
                                       : (HD == 64 ? 4 : HD == 128 ? 3 : 2);
   // byte of a K (or V) step's 16-byte chunk `chunk` of row `row`
@@ -332,8 +337,8 @@ struct Row {   // what a CTA works on: a row's query heads h0 .. h0 + heads - 1 
 
 // One split of a row. phase: steps that this warp's barriers have seen. False if a copy did not come in time.
 template <typename T, int HD, int NT, bool WHOLE>
-__device__ __forceinline__ bool decode_split(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV, uint8_t* smem,
-                                             const Row& row, int split, uint32_t phase) {
+__device__ __forceinline__ bool decode_split(const Params& p, const CUtensorMap* tmK, const CUtensorMap* tmV,
+                                             uint8_t* smem, const Row& row, int split, uint32_t phase) {
   using G = Geo<T, HD, NT, WHOLE>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, tl = lane & 3;
   const int64_t r = row.r, n_vis = row.n_vis, per = row.per, begin = split * per;
@@ -384,7 +389,8 @@ __device__ __forceinline__ bool decode_split(const Params& p, const CUtensorMap*
   // One warp's tiles of a step by TMA: rows past the map's end (bad blocks, tiles past the last key) read as zeros.
   auto load_boxes = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, const int64_t* a) {
     if (lane == 0) {
-      const int row0 = a[0] < 0 ? p.map_rows : static_cast<int>(a[0]), row1 = a[1] < 0 ? p.map_rows : static_cast<int>(a[1]);
+      const int row0 = a[0] < 0 ? p.map_rows : static_cast<int>(a[0]);
+      const int row1 = a[1] < 0 ? p.map_rows : static_cast<int>(a[1]);
       fence_proxy_async_smem();   // the warp's reads of the step that lay there come first
       mbar_arrive_expect_tx(bar, G::STEP_BYTES);
 #pragma unroll
@@ -819,7 +825,8 @@ __global__ void __launch_bounds__(32 * WARPS, Geo<T, HD, NT, WHOLE>::CTAS)
   if (blockIdx.x * row.per >= row.n_vis) {   // the join does not read an empty split
     if (p.splits == 1)                       // a row that sees nothing
       for (int i = threadIdx.x; i < row.heads * p.hd; i += blockDim.x)
-        static_cast<T*>(p.out)[row.r * p.ldo + static_cast<int64_t>(row.kvh * p.rep + row.h0) * p.hd + i] = from_f<T>(0.f);
+        static_cast<T*>(p.out)[row.r * p.ldo + static_cast<int64_t>(row.kvh * p.rep + row.h0) * p.hd + i] =
+            from_f<T>(0.f);
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -869,8 +876,10 @@ int launch_geo(Params p, int64_t B, int64_t nkv, cudaStream_t st) {
   if constexpr (WHOLE) {
     p.rows_per_block = static_cast<int>(p.kv.block_stride / p.hd);
     p.rows_per_head = static_cast<int>(p.kv.head_stride / p.hd);
-    p.map_rows = static_cast<int>((p.kv.num_blocks - 1) * p.rows_per_block + (nkv - 1) * p.rows_per_head + p.kv.block_size);
-    if (make_byte_map(&mk, p.kv.k, p.hd, p.map_rows, TILE) || make_byte_map(&mv, p.kv.v, p.hd, p.map_rows, TILE)) return -1;
+    p.map_rows = static_cast<int>((p.kv.num_blocks - 1) * p.rows_per_block + (nkv - 1) * p.rows_per_head +
+                                  p.kv.block_size);
+    if (make_byte_map(&mk, p.kv.k, p.hd, p.map_rows, TILE) || make_byte_map(&mv, p.kv.v, p.hd, p.map_rows, TILE))
+      return -1;
   }
   static bool attr[64] = {false};
   int dev = 0;

@@ -211,11 +211,12 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float* x, float in
     *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 
-// The vector form, for heads of whole 16-byte pieces (write_vec_ok). A thread owns two pieces of VEC values
-// of a head, chosen so that the lanes of a head read neighbouring pieces: x[VEC c ..] and x[r/2 + VEC c ..] where they turn
-// as pairs (half layout), the same in the copied rest; first and second half of the head otherwise. It does so for HEADS
-// neighbouring heads, so that its cos and sin are read once and its loads are in flight together. The lanes of a head (a power of two,
-// some idle where hd / (2 VEC) is none) find the largest |x| by shuffles.
+// The vector form, for heads of whole 16-byte pieces (write_vec_ok). A thread owns two pieces of VEC values of a head,
+// chosen so that the lanes of a head read neighbouring pieces: x[VEC c ..] and x[r/2 + VEC c ..] where they turn as pairs
+// (half layout), the same in the copied rest; first and second half of the head otherwise. It does so for HEADS
+// neighbouring heads, so that its cos and sin are read once and its loads are in flight together. The lanes of a head (a
+// power of two, some idle where hd / (2 VEC) is none) find the largest |x| by shuffles. The position comes first: a
+// padding token's values are not read.
 template <typename T, bool QUANT, bool IL, int HEADS>
 __global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p, int lanes, unsigned groups) {
   pdl_trigger();
@@ -251,8 +252,8 @@ __global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p,
     T* q_row = static_cast<T*>(p.q_out) + tok * p.ldq;
     Slot at = {-1, -1};
     if (ok && h0 + HEADS > p.nh) at = find_slot(p, tok, pos, c == 0 && h0 <= p.nh);
-    // cos and sin of the thread's VEC pairs. Pairs past the rotated ones are left alone (not turned by 1 and 0: a NaN or an
-    // infinity stays in its own value).
+    // cos and sin of the thread's VEC pairs. Pairs past the rotated ones are left alone (not turned by 1 and 0: a NaN or
+    // an infinity stays in its own value).
     float cs[VEC], sn[VEC];
     auto pair_of = [&](int i) { return IL ? (i < VEC / 2 ? lo / 2 + i : hi / 2 + i - VEC / 2) : VEC * c + i; };
     const float* ct = p.cos_t + pos * half;
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p,
       float x[2 * VEC];
       unpack_piece(raw[u][0], x, static_cast<const T*>(nullptr));
       unpack_piece(raw[u][1], x + VEC, static_cast<const T*>(nullptr));
-      if (!v && turns) {
+      if (mine && !v && turns) {   // a lane without pieces has no cos and sin, and adds zeros to the row's largest value
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           float& a = x[IL ? 2 * i : i];
@@ -433,8 +434,10 @@ int write_t(const WriteParams& p, bool quant, int interleaved, cudaStream_t st) 
     constexpr int HEADS = sizeof(T) == 4 ? 4 : 2;
     const unsigned groups = (p.nh + 2 * p.nkv + HEADS - 1) / HEADS;
     const int64_t vec_blocks = (p.tokens * groups * lanes + 255) / 256;
-    auto kernel = quant ? (interleaved ? rotary_write_vec_kernel<T, true, true, HEADS> : rotary_write_vec_kernel<T, true, false, HEADS>)
-                        : (interleaved ? rotary_write_vec_kernel<T, false, true, HEADS> : rotary_write_vec_kernel<T, false, false, HEADS>);
+    auto kernel = quant ? (interleaved ? rotary_write_vec_kernel<T, true, true, HEADS>
+                                       : rotary_write_vec_kernel<T, true, false, HEADS>)
+                        : (interleaved ? rotary_write_vec_kernel<T, false, true, HEADS>
+                                       : rotary_write_vec_kernel<T, false, false, HEADS>);
     const int64_t ctas = 148 * 4 * (sizeof(T) == 4 ? 4 : 1);
     launch_pdl_async(kernel, static_cast<unsigned>(vec_blocks < ctas ? vec_blocks : ctas), 256, 0, st, p, lanes, groups);
     return check_launch("rotary_write_vec_kernel");

@@ -292,8 +292,8 @@ def _check_quant_cache(kv: L.KVQuantDesc, B: int, nkv: int, hd: int, device: tor
     about = getattr(kv, "about", None)
     if about is not None and (about[0] != device or about[1] != nkv or about[2] != hd or about[3] < B):
         _on_device(device, kv.keep[0])
-        raise ValueError(f"the cache holds {about[1]} heads of {about[2]} for {about[3]} rows, the call has {nkv} of {hd} "
-                         f"for {B}")
+        raise ValueError(f"the cache holds {about[1]} heads of {about[2]} for {about[3]} rows, the call has {nkv} of "
+                         f"{hd} for {B}")
 
 
 def _run(what: str, fn, device: torch.device, *args) -> None:
@@ -465,8 +465,8 @@ def quant_paged_desc(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_
     if v.device != dev or k_scale.device != dev or v_scale.device != dev or table.device != dev:
         _on_device(dev, v, k_scale, v_scale, table)
     desc = L.KVQuantDesc.from_buffer_copy(_PACK_QUANT(
-        k.data_ptr(), v.data_ptr(), table.data_ptr(), t0, width, bs, s0, s1, nblk, k_scale.data_ptr(), v_scale.data_ptr(),
-        c0, c1))
+        k.data_ptr(), v.data_ptr(), table.data_ptr(), t0, width, bs, s0, s1, nblk, k_scale.data_ptr(),
+        v_scale.data_ptr(), c0, c1))
     desc.keep = (k, v, table, k_scale, v_scale)
     desc.about = (dev, nkv, hd, n)
     return desc

@@ -81,6 +81,12 @@ WRITE_CASES = [  # dtype, layout, B, T, nh, nkv, hd, rd, bs
     (torch.float32, "interleaved", 1, 40, 2, 2, 112, 30, 20),
     (torch.float32, "half", 1, 5, 3, 3, 18, 6, 2),
     (torch.bfloat16, "half", 2, 600, 32, 8, 128, 128, 16),
+    # heads whose lanes are no power of two: some hold nothing
+    (torch.bfloat16, "interleaved", 3, 50, 6, 3, 96, 96, 16),
+    (torch.bfloat16, "interleaved", 3, 50, 6, 3, 48, 24, 16),
+    (torch.bfloat16, "half", 3, 50, 5, 5, 112, 64, 16),
+    (torch.float32, "interleaved", 3, 50, 6, 3, 80, 80, 16),
+    (torch.float32, "half", 3, 50, 7, 1, 176, 176, 16),
 ]
 
 
@@ -433,6 +439,23 @@ def test_decode_special_values(dtype, hd):
     q[5] = 0.0
     out = check_decode(q, pools, table, positions, n_slots, nh, nkv, hd)
     assert not out[0].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [128, 40])
+def test_decode_nan_and_infinity_in_a_query_stay_in_their_head(dtype, hd):
+    q, pools, table, positions, n_slots = decode_case(dtype, [600, 40, 9], 8, 2, hd, 16)
+    want, bound = (x.view(3, 8, hd) for x in decode_ref(q, *pools, table, positions, n_slots, 8, 2, hd))
+    bad = q.clone().view(3, 8, hd)
+    bad[0, 1, 3], bad[1, 6, 0], bad[2, 4, hd - 1] = math.nan, math.inf, -math.inf
+    out = torch.empty_like(q)
+    ops.attention_decode_quant(bad.view(3, -1), ops.quant_paged_desc(*pools, table), n_slots, positions, out, 3, 8, 2, hd)
+    out = out.double().view(3, 8, hd)
+    hit = torch.zeros(3, 8, dtype=torch.bool, device=DEV)
+    hit[0, 1] = hit[1, 6] = hit[2, 4] = True
+    assert torch.isnan(out[hit]).all()
+    tol = HALF[dtype] * (want.abs() + bound) + bound
+    assert ((out - want).abs() <= tol)[~hit].all()
 
 
 def test_decode_bad_block_is_flagged_and_reads_zero():
