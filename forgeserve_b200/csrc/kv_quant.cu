@@ -69,8 +69,8 @@ __device__ __forceinline__ bool token_ok(const WriteParams& p, int64_t pos, bool
   return true;
 }
 
-// One warp a (token, head), any even hd up to 512 and any alignment. A lane owns whole pairs (the rotated ones, then
-// neighbours of the copied rest), so a head may be rewritten in place.
+// What the vector form below does not take: one warp a (token, head), any even hd up to 512 and any alignment. A lane
+// owns whole pairs (the rotated ones, then neighbours of the copied rest), so a head may be rewritten in place.
 template <typename T, bool QUANT>
 __global__ void __launch_bounds__(256) rotary_write_kernel(WriteParams p, int interleaved) {
   pdl_trigger();
@@ -181,6 +181,11 @@ __device__ __forceinline__ void load_floats(const float* p, float* x) {
     for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(p + i);
   }
 }
+template <int N>
+__device__ __forceinline__ void put_floats(float* p, const float* x) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = *reinterpret_cast<const float4*>(x + i);
+}
 // N (4 or 8) codes, and their values.
 template <int N>
 __device__ __forceinline__ uint2 load_codes(const uint8_t* p) {
@@ -217,19 +222,32 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float* x, float in
 // neighbouring heads, so that its cos and sin are read once and its loads are in flight together. The lanes of a head (a
 // power of two, some idle where hd / (2 VEC) is none) find the largest |x| by shuffles. The position comes first: a
 // padding token's values are not read.
-template <typename T, bool QUANT, bool IL, int HEADS>
-__global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p, int lanes, unsigned groups) {
+//
+// PAIRS says how a value finds the other one of its pair: HALVES, in the thread's other piece (half layout, r a multiple
+// of 2 VEC); NEIGHBOURS, in the same piece (interleaved layout); STAGED, anywhere in the head (half layout, any r), by way
+// of shared memory, where the lanes take a head's pairs in turn (neighbouring ones at a time, so that tables and banks are
+// read in order; 8192 tokens of 32 + 8 + 8 heads of 128, 126 turned: 60 us to the 8-bit cache, 55 to the bf16 one, 67 in
+// fp32, where a warp a head, as above, takes 178, 171 and 197; every value looking its partner up: 75, 61 and 79).
+enum Pairs { HALVES, NEIGHBOURS, STAGED };
+template <typename T>
+constexpr int WRITE_HEADS = sizeof(T) == 4 ? 4 : 2;   // heads a thread (write_t says why)
+template <Pairs PAIRS>
+constexpr int WRITE_CTAS = PAIRS == STAGED ? 3 : 4;   // CTAs an SM (STAGED: 4 spill, fp32 74 us instead of 67)
+template <typename T, bool QUANT, Pairs PAIRS>
+__global__ void __launch_bounds__(256, WRITE_CTAS<PAIRS>)
+    rotary_write_vec_kernel(WriteParams p, int lanes, unsigned groups) {
   pdl_trigger();
   pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
-  constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T)), HEADS = WRITE_HEADS<T>;
+  constexpr bool IL = PAIRS == NEIGHBOURS;
   const int c = threadIdx.x & (lanes - 1), heads = p.nh + 2 * p.nkv, half = p.rd / 2;
   const unsigned per = 256u / lanes, items = static_cast<unsigned>(p.tokens) * groups;
   // Where the pieces of q and k heads lie, and of v heads.
-  const bool turns = IL || c * 2 * VEC < p.rd;       // IL: pair by pair below,
-  const bool all_turn = !IL || p.rd == p.hd;         // unless all do
+  const bool turns = PAIRS != HALVES || c * 2 * VEC < p.rd;   // IL: pair by pair below,
+  const bool all_turn = !IL || p.rd == p.hd;                  // unless all do
   int lo = VEC * c, hi = p.hd / 2 + VEC * c;
   const int lo_v = lo, hi_v = hi;
-  if (!IL) {
+  if constexpr (PAIRS == HALVES) {
     if (turns) {
       hi = half + VEC * c;
     } else {
@@ -237,6 +255,12 @@ __global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p,
       hi = lo + (p.hd - p.rd) / 2;
     }
   }
+  // STAGED: HEADS heads of values for the lanes of a head (`active` of them own pieces), a warp's groups of lanes apart by
+  // as many banks as they have lanes.
+  __shared__ __align__(16) float staged[PAIRS == STAGED ? 256 * HEADS * 2 * VEC + 1024 : 1];
+  const int group_floats = lanes * HEADS * 2 * VEC + (lanes < 4 ? 4 : lanes);
+  float* const stage = staged + (PAIRS == STAGED ? threadIdx.x / lanes * group_floats : 0);
+  const int active = p.hd / (2 * VEC);
   // Items are (token, HEADS heads). All lanes of a warp stay until its last item is done.
   const unsigned step = gridDim.x * per;
   unsigned item = blockIdx.x * per + threadIdx.x / lanes;
@@ -258,7 +282,11 @@ __global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p,
     auto pair_of = [&](int i) { return IL ? (i < VEC / 2 ? lo / 2 + i : hi / 2 + i - VEC / 2) : VEC * c + i; };
     const float* ct = p.cos_t + pos * half;
     const float* st = p.sin_t + pos * half;
-    if (!IL) {
+    if constexpr (PAIRS == STAGED) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (ok && c + active * i < half) cs[i] = ct[c + active * i], sn[i] = st[c + active * i];
+    } else if constexpr (PAIRS == HALVES) {
       if (ok && turns) {
         load_floats<VEC>(ct + VEC * c, cs);
         load_floats<VEC>(st + VEC * c, sn);
@@ -287,14 +315,47 @@ __global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p,
         raw[u][1] = *reinterpret_cast<const uint4*>(row + h * p.hd + (v ? hi_v : hi));
       }
     }
+    if constexpr (PAIRS == STAGED) {
+      // A lane's own pieces go in and come out; between the barriers the pairs turn where they lie.
+#pragma unroll
+      for (int u = 0; u < HEADS; ++u) {
+        float x[2 * VEC];
+        unpack_piece(raw[u][0], x, static_cast<const T*>(nullptr));
+        unpack_piece(raw[u][1], x + VEC, static_cast<const T*>(nullptr));
+        if (ok) {
+          put_floats<VEC>(stage + u * lanes * 2 * VEC + lo, x);
+          put_floats<VEC>(stage + u * lanes * 2 * VEC + hi, x + VEC);
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < HEADS; ++u) {
+        float* s = stage + u * lanes * 2 * VEC + c;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          if (ok && h0 + u < p.nh + p.nkv && c + active * i < half) {
+            const float a0 = s[active * i], b0 = s[active * i + half];
+            s[active * i] = a0 * cs[i] - b0 * sn[i];
+            s[active * i + half] = b0 * cs[i] + a0 * sn[i];
+          }
+        }
+      }
+      __syncwarp();
+    }
 #pragma unroll
     for (int u = 0; u < HEADS; ++u) {
       const int h = h0 + u;
       const bool v = h >= p.nh + p.nkv, mine = ok && h < heads;
       float x[2 * VEC];
-      unpack_piece(raw[u][0], x, static_cast<const T*>(nullptr));
-      unpack_piece(raw[u][1], x + VEC, static_cast<const T*>(nullptr));
-      if (mine && !v && turns) {   // a lane without pieces has no cos and sin, and adds zeros to the row's largest value
+      if (PAIRS == STAGED && ok) {
+        load_floats<VEC>(stage + u * lanes * 2 * VEC + lo, x);
+        load_floats<VEC>(stage + u * lanes * 2 * VEC + hi, x + VEC);
+      } else {
+        unpack_piece(raw[u][0], x, static_cast<const T*>(nullptr));
+        unpack_piece(raw[u][1], x + VEC, static_cast<const T*>(nullptr));
+      }
+      // a lane without pieces has no cos and sin, and adds zeros to the row's largest value
+      if (PAIRS != STAGED && mine && !v && turns) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           float& a = x[IL ? 2 * i : i];
@@ -336,12 +397,11 @@ __global__ void __launch_bounds__(256, 4) rotary_write_vec_kernel(WriteParams p,
   }
 }
 
-// Whole 16-byte pieces everywhere: heads of 2 VEC values' multiples (the rotated part too, in the half layout), rows,
-// tables and cache on their boundaries.
+// Whole 16-byte pieces everywhere: heads of 2 VEC values' multiples, rows, tables and cache on their boundaries.
 template <typename T>
-bool write_vec_ok(const WriteParams& p, bool quant, bool il) {
+bool write_vec_ok(const WriteParams& p, bool quant) {
   constexpr int VEC = 16 / static_cast<int>(sizeof(T));
-  if (p.hd % (2 * VEC) || p.hd > 64 * VEC || (!il && p.rd % (2 * VEC))) return false;
+  if (p.hd % (2 * VEC) || p.hd > 64 * VEC ) return false;
   const int64_t el = quant ? 16 : VEC;   // elements of the cache in 16 bytes
   if (p.ld % VEC || (p.nh > 0 && p.ldq % VEC) || p.kv.block_stride % el || p.kv.head_stride % el) return false;
   if (quant && p.hd % 16) return false;
@@ -427,19 +487,27 @@ int write_t(const WriteParams& p, bool quant, int interleaved, cudaStream_t st) 
   int lanes = 1;
   while (lanes * PIECES < p.hd) lanes *= 2;
   const int64_t vec_items = p.tokens * ((p.nh + 2 * p.nkv + 1) / 2) * lanes;   // thread numbers of 31 bits (two heads each)
-  if (write_vec_ok<T>(p, quant, interleaved) && vec_items <= INT32_MAX) {
+  if (write_vec_ok<T>(p, quant) && vec_items <= INT32_MAX) {
     // bf16: two heads a thread and one wave of CTAs that stay (8192 tokens of 32 + 8 + 8 heads into the 8-bit cache: 35 us,
     // 41 with a CTA for every 256 threads of work; four heads 40, 88 % of HBM to the bf16 cache). fp32 moves twice the
     // bytes with half the arithmetic: four heads and four waves (58 us, 94 %; one wave 64).
-    constexpr int HEADS = sizeof(T) == 4 ? 4 : 2;
+    constexpr int HEADS = WRITE_HEADS<T>;
     const unsigned groups = (p.nh + 2 * p.nkv + HEADS - 1) / HEADS;
     const int64_t vec_blocks = (p.tokens * groups * lanes + 255) / 256;
-    auto kernel = quant ? (interleaved ? rotary_write_vec_kernel<T, true, true, HEADS>
-                                       : rotary_write_vec_kernel<T, true, false, HEADS>)
-                        : (interleaved ? rotary_write_vec_kernel<T, false, true, HEADS>
-                                       : rotary_write_vec_kernel<T, false, false, HEADS>);
-    const int64_t ctas = 148 * 4 * (sizeof(T) == 4 ? 4 : 1);
-    launch_pdl_async(kernel, static_cast<unsigned>(vec_blocks < ctas ? vec_blocks : ctas), 256, 0, st, p, lanes, groups);
+    auto launch = [&](auto kernel, int per_sm) {
+      const int64_t ctas = 148 * per_sm * (sizeof(T) == 4 ? 4 : 1);
+      launch_pdl_async(kernel, static_cast<unsigned>(vec_blocks < ctas ? vec_blocks : ctas), 256, 0, st, p, lanes,
+                       groups);
+    };
+    if (interleaved)
+      launch(quant ? rotary_write_vec_kernel<T, true, NEIGHBOURS> : rotary_write_vec_kernel<T, false, NEIGHBOURS>,
+             WRITE_CTAS<NEIGHBOURS>);
+    else if (p.rd % PIECES == 0)
+      launch(quant ? rotary_write_vec_kernel<T, true, HALVES> : rotary_write_vec_kernel<T, false, HALVES>,
+             WRITE_CTAS<HALVES>);
+    else
+      launch(quant ? rotary_write_vec_kernel<T, true, STAGED> : rotary_write_vec_kernel<T, false, STAGED>,
+             WRITE_CTAS<STAGED>);
     return check_launch("rotary_write_vec_kernel");
   }
   const int64_t warps = p.tokens * (p.nh + 2 * p.nkv), blocks = (warps + 7) / 8;

@@ -87,6 +87,15 @@ WRITE_CASES = [  # dtype, layout, B, T, nh, nkv, hd, rd, bs
     (torch.bfloat16, "half", 3, 50, 5, 5, 112, 64, 16),
     (torch.float32, "interleaved", 3, 50, 6, 3, 80, 80, 16),
     (torch.float32, "half", 3, 50, 7, 1, 176, 176, 16),
+    # halves that are no whole pieces
+    (torch.bfloat16, "half", 3, 50, 8, 2, 128, 126, 16),
+    (torch.bfloat16, "half", 3, 50, 6, 3, 80, 40, 8),
+    (torch.bfloat16, "half", 2, 33, 5, 1, 512, 2, 16),
+    (torch.bfloat16, "half", 5, 20, 7, 7, 16, 14, 4),
+    (torch.float32, "half", 3, 50, 5, 5, 32, 30, 16),
+    (torch.float32, "half", 2, 21, 3, 1, 256, 254, 16),
+    (torch.float32, "half", 2, 21, 6, 2, 112, 12, 20),
+    (torch.bfloat16, "half", 2, 600, 32, 8, 128, 100, 16),
 ]
 
 
