@@ -171,6 +171,12 @@ __device__ __forceinline__ void store_piece(__nv_bfloat16* p, const float* x) {
 __device__ __forceinline__ void store_piece(float* p, const float* x) {
   *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
 }
+// max(|a|, |b|, |c|), NaN if one of them is.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // N (2, 4 or 8) table values, N-aligned.
 template <int N>
 __device__ __forceinline__ void load_floats(const float* p, float* x) {
@@ -216,73 +222,64 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float* x, float in
     *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 
-// The vector form, for heads of whole 16-byte pieces (write_vec_ok). A thread owns two pieces of VEC values of a head,
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {   // to shared memory
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// The vector forms, for heads of whole 16-byte pieces (write_vec_ok). A thread owns two pieces of VEC values of a head,
 // chosen so that the lanes of a head read neighbouring pieces: x[VEC c ..] and x[r/2 + VEC c ..] where they turn as pairs
 // (half layout), the same in the copied rest; first and second half of the head otherwise. It does so for HEADS
-// neighbouring heads, so that its cos and sin are read once and its loads are in flight together. The lanes of a head (a
-// power of two, some idle where hd / (2 VEC) is none) find the largest |x| by shuffles. The position comes first: a
-// padding token's values are not read.
+// neighbouring heads, so that its cos and sin are read once. The lanes of a head (a power of two, some idle where
+// hd / (2 VEC) is none) find the largest |x| by shuffles. The position comes first: a padding token's values are not read.
 //
 // PAIRS says how a value finds the other one of its pair: HALVES, in the thread's other piece (half layout, r a multiple
-// of 2 VEC); NEIGHBOURS, in the same piece (interleaved layout); STAGED, anywhere in the head (half layout, any r), by way
-// of shared memory, where the lanes take a head's pairs in turn (neighbouring ones at a time, so that tables and banks are
-// read in order; 8192 tokens of 32 + 8 + 8 heads of 128, 126 turned: 60 us to the 8-bit cache, 55 to the bf16 one, 67 in
-// fp32, where a warp a head, as above, takes 178, 171 and 197; every value looking its partner up: 75, 61 and 79).
+// of 2 VEC); NEIGHBOURS, in the same piece (interleaved layout); STAGED, anywhere in the head (half layout, any r).
+//
+// One wave of CTAs stays, and a thread copies its next item's pieces into shared memory while it works on one (8 ragged
+// rows of 2048 tokens of 64 + 8 + 8 heads of 128 to the 8-bit cache: 91 us, 96 % of HBM; loads into registers 105, the
+// issue slots being 62 % busy while nothing hides a load). Three CTAs an SM hold all in registers; four spill and put
+// more streams on HBM (91 -> 95; fp32 55 -> 62 for 8192 tokens of 32 + 8 + 8 heads).
 enum Pairs { HALVES, NEIGHBOURS, STAGED };
 template <typename T>
-constexpr int WRITE_HEADS = sizeof(T) == 4 ? 4 : 2;   // heads a thread (write_t says why)
-template <Pairs PAIRS>
-constexpr int WRITE_CTAS = PAIRS == STAGED ? 3 : 4;   // CTAs an SM (STAGED: 4 spill, fp32 74 us instead of 67)
-template <typename T, bool QUANT, Pairs PAIRS>
-__global__ void __launch_bounds__(256, WRITE_CTAS<PAIRS>)
-    rotary_write_vec_kernel(WriteParams p, int lanes, unsigned groups) {
-  pdl_trigger();
-  pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
-  constexpr int VEC = 16 / static_cast<int>(sizeof(T)), HEADS = WRITE_HEADS<T>;
-  constexpr bool IL = PAIRS == NEIGHBOURS;
-  const int c = threadIdx.x & (lanes - 1), heads = p.nh + 2 * p.nkv, half = p.rd / 2;
-  const unsigned per = 256u / lanes, items = static_cast<unsigned>(p.tokens) * groups;
-  // Where the pieces of q and k heads lie, and of v heads.
-  const bool turns = PAIRS != HALVES || c * 2 * VEC < p.rd;   // IL: pair by pair below,
-  const bool all_turn = !IL || p.rd == p.hd;                  // unless all do
-  int lo = VEC * c, hi = p.hd / 2 + VEC * c;
-  const int lo_v = lo, hi_v = hi;
-  if constexpr (PAIRS == HALVES) {
-    if (turns) {
-      hi = half + VEC * c;
-    } else {
-      lo = p.rd + VEC * c - half;   // c - rd / (2 VEC) pieces into the rest
-      hi = lo + (p.hd - p.rd) / 2;
+constexpr int VALUES = 16 / static_cast<int>(sizeof(T));   // VEC: values of a piece
+constexpr int WRITE_HEADS = 2, WRITE_CTAS = 3;             // HEADS; CTAs an SM
+
+// A lane's place in a head: where its pieces lie, of q and k heads and of v heads.
+template <typename T, Pairs PAIRS>
+struct Lane {
+  static constexpr int VEC = VALUES<T>;
+  static constexpr bool IL = PAIRS == NEIGHBOURS;
+  int c, lanes, half, heads, lo, hi, lo_v, hi_v;
+  bool owns, turns, all_turn;
+  __device__ __forceinline__ Lane(const WriteParams& p, int n) {
+    lanes = n;
+    c = threadIdx.x & (lanes - 1);
+    half = p.rd / 2;
+    heads = p.nh + 2 * p.nkv;
+    owns = c * 2 * VEC < p.hd;
+    turns = PAIRS != HALVES || c * 2 * VEC < p.rd;   // IL: pair by pair below,
+    all_turn = !IL || p.rd == p.hd;                  // unless all do
+    lo = lo_v = VEC * c;
+    hi = hi_v = p.hd / 2 + VEC * c;
+    if constexpr (PAIRS == HALVES) {
+      if (turns) {
+        hi = half + VEC * c;
+      } else {
+        lo = p.rd + VEC * c - half;   // c - rd / (2 VEC) pieces into the rest
+        hi = lo + (p.hd - p.rd) / 2;
+      }
     }
   }
-  // STAGED: HEADS heads of values for the lanes of a head (`active` of them own pieces), a warp's groups of lanes apart by
-  // as many banks as they have lanes.
-  __shared__ __align__(16) float staged[PAIRS == STAGED ? 256 * HEADS * 2 * VEC + 1024 : 1];
-  const int group_floats = lanes * HEADS * 2 * VEC + (lanes < 4 ? 4 : lanes);
-  float* const stage = staged + (PAIRS == STAGED ? threadIdx.x / lanes * group_floats : 0);
-  const int active = p.hd / (2 * VEC);
-  // Items are (token, HEADS heads). All lanes of a warp stay until its last item is done.
-  const unsigned step = gridDim.x * per;
-  unsigned item = blockIdx.x * per + threadIdx.x / lanes;
-  int64_t next_pos = item < items ? p.positions[item / groups] : -1;
-  while (__any_sync(0xffffffffu, item < items)) {
-    const unsigned token = item / groups;
-    const int h0 = (item - token * groups) * HEADS;
-    const int64_t tok = token, pos = next_pos;
-    const bool ok = item < items && c * 2 * VEC < p.hd && token_ok(p, pos, c == 0 && h0 == 0);
-    const unsigned next = item + step;
-    next_pos = next < items ? p.positions[next / groups] : -1;
-    const T* row = static_cast<const T*>(p.qkv) + tok * p.ld;
-    T* q_row = static_cast<T*>(p.q_out) + tok * p.ldq;
-    Slot at = {-1, -1};
-    if (ok && h0 + HEADS > p.nh) at = find_slot(p, tok, pos, c == 0 && h0 <= p.nh);
-    // cos and sin of the thread's VEC pairs. Pairs past the rotated ones are left alone (not turned by 1 and 0: a NaN or
-    // an infinity stays in its own value).
-    float cs[VEC], sn[VEC];
-    auto pair_of = [&](int i) { return IL ? (i < VEC / 2 ? lo / 2 + i : hi / 2 + i - VEC / 2) : VEC * c + i; };
+  __device__ __forceinline__ int pair_of(int i) const {
+    return IL ? (i < VEC / 2 ? lo / 2 + i : hi / 2 + i - VEC / 2) : VEC * c + i;
+  }
+  // cos and sin of the thread's VEC pairs. Pairs past the rotated ones are left alone (not turned by 1 and 0: a NaN or an
+  // infinity stays in its own value).
+  __device__ __forceinline__ void load_turns(const WriteParams& p, bool ok, int64_t pos, float* cs, float* sn) const {
     const float* ct = p.cos_t + pos * half;
     const float* st = p.sin_t + pos * half;
     if constexpr (PAIRS == STAGED) {
+      const int active = p.hd / (2 * VEC);
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
         if (ok && c + active * i < half) cs[i] = ct[c + active * i], sn[i] = st[c + active * i];
@@ -304,96 +301,229 @@ __global__ void __launch_bounds__(256, WRITE_CTAS<PAIRS>)
       for (int i = 0; i < VEC; ++i)
         if (pair_of(i) < half) cs[i] = ct[pair_of(i)], sn[i] = st[pair_of(i)];
     }
+  }
+  // The lane's pairs of a q or k head.
+  __device__ __forceinline__ void turn(float* x, const float* cs, const float* sn) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      float& a = x[IL ? 2 * i : i];
+      float& b = x[IL ? 2 * i + 1 : VEC + i];
+      const float a0 = a, b0 = b;
+      if (!IL || all_turn || pair_of(i) < half) {
+        a = a0 * cs[i] - b0 * sn[i];
+        b = b0 * cs[i] + a0 * sn[i];
+      }
+    }
+  }
+  // Stores the lane's values of head h: q to q_row, k and v to the cache. mine: the head is the lane's; all lanes call.
+  template <bool QUANT>
+  __device__ __forceinline__ void put(const WriteParams& p, bool mine, int h, const float* x, T* q_row,
+                                      const Slot& at) const {
+    const bool v = h >= p.nh + p.nkv;
+    if (mine && h < p.nh) {
+      store_piece(q_row + h * p.hd + lo, x);
+      store_piece(q_row + h * p.hd + hi, x + VEC);
+    }
+    const int g = h - p.nh - (v ? p.nkv : 0);
+    const bool to_cache = mine && h >= p.nh && at.values >= 0;
+    const int l0 = v ? lo_v : lo, l1 = v ? hi_v : hi;
+    if constexpr (QUANT) {
+      if (!__any_sync(0xffffffffu, to_cache)) return;   // a warp of q heads
+      float largest = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * VEC; i += 2) largest = max_abs(largest, x[i], x[i + 1]);
+      uint32_t top = abs_bits(largest);
+      for (int o = lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (to_cache) {
+        const float scale = row_scale(top), inv = inverse(scale);
+        uint8_t* o = static_cast<uint8_t*>(v ? p.kv.v : p.kv.k) + at.values + g * p.kv.head_stride;
+        store_codes<VEC>(o + l0, x, inv);
+        store_codes<VEC>(o + l1, x + VEC, inv);
+        if (c == 0) (v ? p.sc.v : p.sc.k)[at.scale + g * p.sc.head_stride] = scale;
+      }
+    } else if (to_cache) {
+      T* o = static_cast<T*>(v ? p.kv.v : p.kv.k) + at.values + g * p.kv.head_stride;
+      store_piece(o + l0, x);
+      store_piece(o + l1, x + VEC);
+    }
+  }
+};
+
+// Items are (token, HEADS heads); a group of lanes takes every step-th of them. The step moves it on by about 3/8 of a
+// token's items each time (whole warps of them, so that a warp's stay alike): heads for the cache cost more than heads of
+// q, and where the grid is a multiple of a token's items every warp would meet the same heads again and again (16 x 2048
+// tokens of 32 + 8 + 8 heads: 152 us instead of 116).
+struct Items {
+  unsigned count, groups, step, step_tok, step_group, item, token, group;
+  __device__ __forceinline__ Items(const WriteParams& p, int lanes, unsigned n_groups) {
+    const unsigned per = 256u / lanes, warp = 32u / lanes, total = gridDim.x * per;
+    groups = n_groups;
+    count = static_cast<unsigned>(p.tokens) * groups;
+    step = total;
+    if (count > total) {
+      const unsigned on = max(groups * 3 / 8 / warp * warp, warp) % groups;
+      step -= (total + groups - on) % groups;
+    }
+    step_tok = step / groups;
+    step_group = step - step_tok * groups;
+    item = blockIdx.x * per + threadIdx.x / lanes;
+    if (item >= step) item = count;   // the last few, for the step's sake
+    token = item / groups;
+    group = item - token * groups;
+  }
+  __device__ __forceinline__ bool left() const { return item < count; }
+  __device__ __forceinline__ void advance() {
+    item += step;
+    token += step_tok;
+    group += step_group;
+    if (group >= groups) {
+      group -= groups;
+      ++token;
+    }
+  }
+};
+
+template <typename T, bool QUANT, Pairs PAIRS>
+__global__ void __launch_bounds__(256, WRITE_CTAS)
+    rotary_write_vec_kernel(WriteParams p, int lanes, unsigned groups) {
+  pdl_trigger();
+  pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
+  constexpr int VEC = VALUES<T>, HEADS = WRITE_HEADS;
+  __shared__ __align__(16) uint4 ahead[2][HEADS][2][256];
+  const Lane<T, PAIRS> lane(p, lanes);
+  const int c = lane.c, heads = lane.heads;
+  Items it(p, lanes, groups);   // the item ahead
+  auto fetch = [&](int to, int64_t at_pos) {
+    if (it.left() && lane.owns && token_ok(p, at_pos, false)) {
+      const T* row = static_cast<const T*>(p.qkv) + static_cast<int64_t>(it.token) * p.ld;
+#pragma unroll
+      for (int u = 0; u < HEADS; ++u) {
+        const int h = it.group * HEADS + u;
+        const bool v = h >= p.nh + p.nkv;
+        if (h < heads) {
+          copy_async16(&ahead[to][u][0][threadIdx.x], row + h * p.hd + (v ? lane.lo_v : lane.lo));
+          copy_async16(&ahead[to][u][1][threadIdx.x], row + h * p.hd + (v ? lane.hi_v : lane.hi));
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // The item at hand: its token, first head, position and whether there is one; its pieces lie in ahead[buf].
+  unsigned token = it.token;
+  int h0 = it.group * HEADS, buf = 0;
+  bool real = it.left();
+  int64_t pos = real ? p.positions[token] : -1;
+  fetch(0, pos);
+  it.advance();
+  int64_t ahead_pos = it.left() ? p.positions[it.token] : -1;
+  while (__any_sync(0xffffffffu, real)) {   // all lanes of a warp stay until its last item is done
+    const int64_t tok = token;
+    const bool ok = real && lane.owns && token_ok(p, pos, c == 0 && h0 == 0);
+    const unsigned next_token = it.token;
+    const int next_h0 = it.group * HEADS;
+    const int64_t next_pos = ahead_pos;
+    const bool next_real = it.left();
+    T* q_row = static_cast<T*>(p.q_out) + tok * p.ldq;
+    Slot at = {-1, -1};
+    if (ok && h0 + HEADS > p.nh) at = find_slot(p, tok, pos, c == 0 && h0 <= p.nh);
+    float cs[VEC], sn[VEC];
+    lane.load_turns(p, ok, pos, cs, sn);
+    fetch(buf ^ 1, next_pos);
+    it.advance();
+    ahead_pos = it.left() ? p.positions[it.token] : -1;
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < HEADS; ++u) {
+      const int h = h0 + u;
+      const bool mine = ok && h < heads;
+      float x[2 * VEC];
+      const uint4 none = make_uint4(0, 0, 0, 0);   // lanes without pieces add zeros to the row's largest value
+      unpack_piece(mine ? ahead[buf][u][0][threadIdx.x] : none, x, static_cast<const T*>(nullptr));
+      unpack_piece(mine ? ahead[buf][u][1][threadIdx.x] : none, x + VEC, static_cast<const T*>(nullptr));
+      if (mine && h < p.nh + p.nkv && lane.turns) lane.turn(x, cs, sn);
+      lane.template put<QUANT>(p, mine, h, x, q_row, at);
+    }
+    token = next_token;
+    h0 = next_h0;
+    pos = next_pos;
+    real = next_real;
+    buf ^= 1;
+  }
+}
+
+// STAGED: a head's values go through shared memory, where its lanes take the pairs in turn (neighbouring ones at a time,
+// so that tables and banks are read in order). 8192 tokens of 32 + 8 + 8 heads of 128, 126 turned: 53 us to the 8-bit
+// cache, 51 to the bf16 one, 69 in fp32, where a warp a head, as above, takes 178, 171 and 197.
+template <typename T, bool QUANT>
+__global__ void __launch_bounds__(256, WRITE_CTAS)
+    rotary_write_staged_kernel(WriteParams p, int lanes, unsigned groups) {
+  pdl_trigger();
+  pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
+  constexpr int VEC = VALUES<T>, HEADS = WRITE_HEADS;
+  const Lane<T, STAGED> lane(p, lanes);
+  const int c = lane.c, heads = lane.heads;
+  // HEADS heads of values for the lanes of a head (`active` of them own pieces), a warp's groups of lanes apart by as many
+  // banks as they have lanes.
+  __shared__ __align__(16) float staged[256 * HEADS * 2 * VEC + 1024];
+  const int group_floats = lanes * HEADS * 2 * VEC + (lanes < 4 ? 4 : lanes), active = p.hd / (2 * VEC);
+  float* const stage = staged + threadIdx.x / lanes * group_floats;
+  Items it(p, lanes, groups);
+  int64_t next_pos = it.left() ? p.positions[it.token] : -1;
+  while (__any_sync(0xffffffffu, it.left())) {   // all lanes of a warp stay until its last item is done
+    const int h0 = it.group * HEADS;
+    const int64_t tok = it.token, pos = next_pos;
+    const bool ok = it.left() && lane.owns && token_ok(p, pos, c == 0 && h0 == 0);
+    it.advance();
+    next_pos = it.left() ? p.positions[it.token] : -1;
+    const T* row = static_cast<const T*>(p.qkv) + tok * p.ld;
+    T* q_row = static_cast<T*>(p.q_out) + tok * p.ldq;
+    Slot at = {-1, -1};
+    if (ok && h0 + HEADS > p.nh) at = find_slot(p, tok, pos, c == 0 && h0 <= p.nh);
+    float cs[VEC], sn[VEC];
+    lane.load_turns(p, ok, pos, cs, sn);
     uint4 raw[HEADS][2];
 #pragma unroll
     for (int u = 0; u < HEADS; ++u) {
-      const int h = h0 + u;
       raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
-      if (ok && h < heads) {
-        const bool v = h >= p.nh + p.nkv;
-        raw[u][0] = *reinterpret_cast<const uint4*>(row + h * p.hd + (v ? lo_v : lo));
-        raw[u][1] = *reinterpret_cast<const uint4*>(row + h * p.hd + (v ? hi_v : hi));
+      if (ok && h0 + u < heads) {
+        raw[u][0] = *reinterpret_cast<const uint4*>(row + (h0 + u) * p.hd + lane.lo);
+        raw[u][1] = *reinterpret_cast<const uint4*>(row + (h0 + u) * p.hd + lane.hi);
       }
     }
-    if constexpr (PAIRS == STAGED) {
-      // A lane's own pieces go in and come out; between the barriers the pairs turn where they lie.
-#pragma unroll
-      for (int u = 0; u < HEADS; ++u) {
-        float x[2 * VEC];
-        unpack_piece(raw[u][0], x, static_cast<const T*>(nullptr));
-        unpack_piece(raw[u][1], x + VEC, static_cast<const T*>(nullptr));
-        if (ok) {
-          put_floats<VEC>(stage + u * lanes * 2 * VEC + lo, x);
-          put_floats<VEC>(stage + u * lanes * 2 * VEC + hi, x + VEC);
-        }
-      }
-      __syncwarp();
-#pragma unroll
-      for (int u = 0; u < HEADS; ++u) {
-        float* s = stage + u * lanes * 2 * VEC + c;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          if (ok && h0 + u < p.nh + p.nkv && c + active * i < half) {
-            const float a0 = s[active * i], b0 = s[active * i + half];
-            s[active * i] = a0 * cs[i] - b0 * sn[i];
-            s[active * i + half] = b0 * cs[i] + a0 * sn[i];
-          }
-        }
-      }
-      __syncwarp();
-    }
+    // A lane's own pieces go in and come out; between the barriers the pairs turn where they lie.
 #pragma unroll
     for (int u = 0; u < HEADS; ++u) {
-      const int h = h0 + u;
-      const bool v = h >= p.nh + p.nkv, mine = ok && h < heads;
       float x[2 * VEC];
-      if (PAIRS == STAGED && ok) {
-        load_floats<VEC>(stage + u * lanes * 2 * VEC + lo, x);
-        load_floats<VEC>(stage + u * lanes * 2 * VEC + hi, x + VEC);
-      } else {
-        unpack_piece(raw[u][0], x, static_cast<const T*>(nullptr));
-        unpack_piece(raw[u][1], x + VEC, static_cast<const T*>(nullptr));
-      }
-      // a lane without pieces has no cos and sin, and adds zeros to the row's largest value
-      if (PAIRS != STAGED && mine && !v && turns) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          float& a = x[IL ? 2 * i : i];
-          float& b = x[IL ? 2 * i + 1 : VEC + i];
-          const float a0 = a, b0 = b;
-          if (!IL || all_turn || pair_of(i) < half) {
-            a = a0 * cs[i] - b0 * sn[i];
-            b = b0 * cs[i] + a0 * sn[i];
-          }
-        }
-      }
-      if (mine && h < p.nh) {
-        store_piece(q_row + h * p.hd + lo, x);
-        store_piece(q_row + h * p.hd + hi, x + VEC);
-      }
-      const int g = h - p.nh - (v ? p.nkv : 0);
-      const bool put = mine && h >= p.nh && at.values >= 0;
-      const int l0 = v ? lo_v : lo, l1 = v ? hi_v : hi;
-      if constexpr (QUANT) {
-        if (!__any_sync(0xffffffffu, put)) continue;   // a warp of q heads
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 2 * VEC; ++i) top = max(top, abs_bits(x[i]));
-        for (int o = lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (put) {
-          const float scale = row_scale(top), inv = inverse(scale);
-          uint8_t* o = static_cast<uint8_t*>(v ? p.kv.v : p.kv.k) + at.values + g * p.kv.head_stride;
-          store_codes<VEC>(o + l0, x, inv);
-          store_codes<VEC>(o + l1, x + VEC, inv);
-          if (c == 0) (v ? p.sc.v : p.sc.k)[at.scale + g * p.sc.head_stride] = scale;
-        }
-      } else if (put) {
-        T* o = static_cast<T*>(v ? p.kv.v : p.kv.k) + at.values + g * p.kv.head_stride;
-        store_piece(o + l0, x);
-        store_piece(o + l1, x + VEC);
+      unpack_piece(raw[u][0], x, static_cast<const T*>(nullptr));
+      unpack_piece(raw[u][1], x + VEC, static_cast<const T*>(nullptr));
+      if (ok) {
+        put_floats<VEC>(stage + u * lanes * 2 * VEC + lane.lo, x);
+        put_floats<VEC>(stage + u * lanes * 2 * VEC + lane.hi, x + VEC);
       }
     }
-    item = next;
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < HEADS; ++u) {
+      float* s = stage + u * lanes * 2 * VEC + c;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if (ok && h0 + u < p.nh + p.nkv && c + active * i < lane.half) {
+          const float a0 = s[active * i], b0 = s[active * i + lane.half];
+          s[active * i] = a0 * cs[i] - b0 * sn[i];
+          s[active * i + lane.half] = b0 * cs[i] + a0 * sn[i];
+        }
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < HEADS; ++u) {
+      float x[2 * VEC] = {};   // lanes without pieces add zeros to the row's largest value
+      if (ok) {
+        load_floats<VEC>(stage + u * lanes * 2 * VEC + lane.lo, x);
+        load_floats<VEC>(stage + u * lanes * 2 * VEC + lane.hi, x + VEC);
+      }
+      lane.template put<QUANT>(p, ok && h0 + u < heads, h0 + u, x, q_row, at);
+    }
   }
 }
 
@@ -486,28 +616,19 @@ int write_t(const WriteParams& p, bool quant, int interleaved, cudaStream_t st) 
   constexpr int PIECES = 32 / static_cast<int>(sizeof(T));   // values a lane of the vector form holds of a head
   int lanes = 1;
   while (lanes * PIECES < p.hd) lanes *= 2;
-  const int64_t vec_items = p.tokens * ((p.nh + 2 * p.nkv + 1) / 2) * lanes;   // thread numbers of 31 bits (two heads each)
+  const int64_t vec_items = p.tokens * ((p.nh + 2 * p.nkv + 1) / 2) * lanes;   // thread numbers of 31 bits
   if (write_vec_ok<T>(p, quant) && vec_items <= INT32_MAX) {
-    // bf16: two heads a thread and one wave of CTAs that stay (8192 tokens of 32 + 8 + 8 heads into the 8-bit cache: 35 us,
-    // 41 with a CTA for every 256 threads of work; four heads 40, 88 % of HBM to the bf16 cache). fp32 moves twice the
-    // bytes with half the arithmetic: four heads and four waves (58 us, 94 %; one wave 64).
-    constexpr int HEADS = WRITE_HEADS<T>;
-    const unsigned groups = (p.nh + 2 * p.nkv + HEADS - 1) / HEADS;
-    const int64_t vec_blocks = (p.tokens * groups * lanes + 255) / 256;
-    auto launch = [&](auto kernel, int per_sm) {
-      const int64_t ctas = 148 * per_sm * (sizeof(T) == 4 ? 4 : 1);
-      launch_pdl_async(kernel, static_cast<unsigned>(vec_blocks < ctas ? vec_blocks : ctas), 256, 0, st, p, lanes,
-                       groups);
+    const unsigned groups = (p.nh + 2 * p.nkv + WRITE_HEADS - 1) / WRITE_HEADS;
+    const int64_t blocks = (p.tokens * groups * lanes + 255) / 256, wave = 148 * WRITE_CTAS;
+    auto launch = [&](auto kernel) {
+      launch_pdl_async(kernel, static_cast<unsigned>(blocks < wave ? blocks : wave), 256, 0, st, p, lanes, groups);
     };
     if (interleaved)
-      launch(quant ? rotary_write_vec_kernel<T, true, NEIGHBOURS> : rotary_write_vec_kernel<T, false, NEIGHBOURS>,
-             WRITE_CTAS<NEIGHBOURS>);
+      launch(quant ? rotary_write_vec_kernel<T, true, NEIGHBOURS> : rotary_write_vec_kernel<T, false, NEIGHBOURS>);
     else if (p.rd % PIECES == 0)
-      launch(quant ? rotary_write_vec_kernel<T, true, HALVES> : rotary_write_vec_kernel<T, false, HALVES>,
-             WRITE_CTAS<HALVES>);
+      launch(quant ? rotary_write_vec_kernel<T, true, HALVES> : rotary_write_vec_kernel<T, false, HALVES>);
     else
-      launch(quant ? rotary_write_vec_kernel<T, true, STAGED> : rotary_write_vec_kernel<T, false, STAGED>,
-             WRITE_CTAS<STAGED>);
+      launch(quant ? rotary_write_staged_kernel<T, true> : rotary_write_staged_kernel<T, false>);
     return check_launch("rotary_write_vec_kernel");
   }
   const int64_t warps = p.tokens * (p.nh + 2 * p.nkv), blocks = (warps + 7) / 8;
@@ -573,7 +694,8 @@ int kv_dequant(int dtype, const KVCache& kv, const KVScales& sc, int64_t B, int6
                        static_cast<__nv_bfloat16*>(v_out), err, static_cast<unsigned>(chunks), static_cast<unsigned>(total));
     return check_launch("kv_dequant_vec_kernel");
   }
-  const dim3 grid(static_cast<unsigned>((n_slots * hd + 255) / 256), static_cast<unsigned>(nkv), static_cast<unsigned>(B));
+  const dim3 grid(static_cast<unsigned>((n_slots * hd + 255) / 256), static_cast<unsigned>(nkv),
+                  static_cast<unsigned>(B));
   auto run = [&](auto* k, auto* v) {
     using T = std::remove_pointer_t<decltype(k)>;
     launch_pdl_async(kv_dequant_kernel<T>, grid, 256, 0, st, kv, sc, static_cast<uint32_t>(n_slots),

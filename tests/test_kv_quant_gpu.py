@@ -96,6 +96,14 @@ WRITE_CASES = [  # dtype, layout, B, T, nh, nkv, hd, rd, bs
     (torch.float32, "half", 2, 21, 3, 1, 256, 254, 16),
     (torch.float32, "half", 2, 21, 6, 2, 112, 12, 20),
     (torch.bfloat16, "half", 2, 600, 32, 8, 128, 100, 16),
+    # more items than a wave of CTAs takes at once
+    (torch.bfloat16, "half", 3, 1500, 5, 2, 64, 64, 16),
+    (torch.bfloat16, "half", 2, 3000, 40, 8, 16, 16, 16),
+    (torch.bfloat16, "interleaved", 2, 900, 16, 8, 128, 128, 16),
+    (torch.bfloat16, "interleaved", 1, 9000, 1, 1, 128, 64, 32),
+    (torch.float32, "interleaved", 2, 700, 9, 3, 80, 80, 7),
+    (torch.float32, "half", 3, 500, 32, 8, 128, 128, 16),
+    (torch.float32, "half", 2, 800, 11, 1, 64, 62, 16),
 ]
 
 
