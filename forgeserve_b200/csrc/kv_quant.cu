@@ -383,8 +383,8 @@ struct Items {
   }
 };
 
-template <typename T, bool QUANT, Pairs PAIRS>
-__global__ void __launch_bounds__(256, WRITE_CTAS)
+template <typename T, bool QUANT, Pairs PAIRS, int CTAS = WRITE_CTAS>
+__global__ void __launch_bounds__(256, CTAS)
     rotary_write_vec_kernel(WriteParams p, int lanes, unsigned groups) {
   pdl_trigger();
   pdl_wait();   // launched with PDL: everything below reads or writes other kernels' data
@@ -619,16 +619,26 @@ int write_t(const WriteParams& p, bool quant, int interleaved, cudaStream_t st) 
   const int64_t vec_items = p.tokens * ((p.nh + 2 * p.nkv + 1) / 2) * lanes;   // thread numbers of 31 bits
   if (write_vec_ok<T>(p, quant) && vec_items <= INT32_MAX) {
     const unsigned groups = (p.nh + 2 * p.nkv + WRITE_HEADS - 1) / WRITE_HEADS;
-    const int64_t blocks = (p.tokens * groups * lanes + 255) / 256, wave = 148 * WRITE_CTAS;
-    auto launch = [&](auto kernel) {
+    const int64_t blocks = (p.tokens * groups * lanes + 255) / 256;
+    auto launch = [&](auto kernel, int ctas) {
+      const int64_t wave = 148 * ctas;
       launch_pdl_async(kernel, static_cast<unsigned>(blocks < wave ? blocks : wave), 256, 0, st, p, lanes, groups);
     };
-    if (interleaved)
-      launch(quant ? rotary_write_vec_kernel<T, true, NEIGHBOURS> : rotary_write_vec_kernel<T, false, NEIGHBOURS>);
-    else if (p.rd % PIECES == 0)
-      launch(quant ? rotary_write_vec_kernel<T, true, HALVES> : rotary_write_vec_kernel<T, false, HALVES>);
+    // A plain write past L2 (a lane reads 64 bytes an item) takes two CTAs an SM, with registers for more loads at once and
+    // fewer streams on HBM: 16384 tokens of 32 + 8 + 8 heads 65 us against 70 with three, 65536 249 against 281; 8192 34.5
+    // against 33.5. The 8-bit cache's needs the third for its arithmetic (16 x 2048 tokens: 116 us, 130 with two).
+    const bool large = p.tokens * groups * lanes > (int64_t{128} << 20) / 64;
+    if (!interleaved && p.rd % PIECES)
+      launch(quant ? rotary_write_staged_kernel<T, true> : rotary_write_staged_kernel<T, false>, WRITE_CTAS);
+    else if (quant)
+      launch(interleaved ? rotary_write_vec_kernel<T, true, NEIGHBOURS> : rotary_write_vec_kernel<T, true, HALVES>,
+             WRITE_CTAS);
+    else if (!large)
+      launch(interleaved ? rotary_write_vec_kernel<T, false, NEIGHBOURS> : rotary_write_vec_kernel<T, false, HALVES>,
+             WRITE_CTAS);
     else
-      launch(quant ? rotary_write_staged_kernel<T, true> : rotary_write_staged_kernel<T, false>);
+      launch(interleaved ? rotary_write_vec_kernel<T, false, NEIGHBOURS, 2> : rotary_write_vec_kernel<T, false, HALVES, 2>,
+             2);
     return check_launch("rotary_write_vec_kernel");
   }
   const int64_t warps = p.tokens * (p.nh + 2 * p.nkv), blocks = (warps + 7) / 8;
