@@ -360,7 +360,7 @@ struct Items {
     groups = n_groups;
     count = static_cast<unsigned>(p.tokens) * groups;
     step = total;
-    if (count > total) {
+    if (count > total && total > groups) {
       const unsigned on = max(groups * 3 / 8 / warp * warp, warp) % groups;
       step -= (total + groups - on) % groups;
     }
