@@ -104,6 +104,9 @@ WRITE_CASES = [  # dtype, layout, B, T, nh, nkv, hd, rd, bs
     (torch.float32, "interleaved", 2, 700, 9, 3, 80, 80, 7),
     (torch.float32, "half", 3, 500, 32, 8, 128, 128, 16),
     (torch.float32, "half", 2, 800, 11, 1, 64, 62, 16),
+    (torch.bfloat16, "half", 3, 700, 12, 4, 208, 208, 16),
+    (torch.bfloat16, "half", 3, 700, 12, 4, 272, 270, 16),
+    (torch.float32, "interleaved", 3, 700, 6, 2, 24, 24, 16),
     # past 128 MiB of rows
     (torch.bfloat16, "half", 3, 3500, 40, 8, 128, 128, 64),
     (torch.float32, "interleaved", 1, 4700, 40, 9, 128, 64, 64),
