@@ -771,8 +771,10 @@ __device__ __forceinline__ bool decode_split(const Params& p, const CUtensorMap*
       total += f[w] * msm[2 * (w * 8 * NT + h) + 1];
     }
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) wsm[h * WARPS + w] = p.splits == 1 ? f[w] / total : f[w];
-    if (p.splits > 1) {
+    for (int w = 0; w < WARPS; ++w) wsm[h * WARPS + w] = f[w];
+    if (p.splits == 1) {
+      msm[2 * h] = total;   // over warp 0's maximum, which this thread alone has read
+    } else {
       float* ml = p.ws + static_cast<int64_t>(gridDim.z) * p.nh * p.splits * p.hd +
                   2 * (part0 + static_cast<int64_t>(h) * p.splits);
       ml[0] = top;
@@ -793,12 +795,13 @@ __device__ __forceinline__ bool decode_split(const Params& p, const CUtensorMap*
       o.z = fmaf(f, x.z, o.z);
       o.w = fmaf(f, x.w, o.w);
     }
-    if (p.splits == 1) {
+    if (p.splits == 1) {   // divided after the sum, as the join divides: a row's only split gives the same bits there
       T* dst = static_cast<T*>(p.out) + r * p.ldo + static_cast<int64_t>(kvh * p.rep + h0 + h) * p.hd + d;
-      dst[0] = from_f<T>(o.x);
-      dst[1] = from_f<T>(o.y);
-      dst[2] = from_f<T>(o.z);
-      dst[3] = from_f<T>(o.w);
+      const float total = msm[2 * h];
+      dst[0] = from_f<T>(o.x / total);
+      dst[1] = from_f<T>(o.y / total);
+      dst[2] = from_f<T>(o.z / total);
+      dst[3] = from_f<T>(o.w / total);
     } else {
       *reinterpret_cast<float4*>(p.ws + (part0 + static_cast<int64_t>(h) * p.splits) * p.hd + d) = o;
     }

@@ -831,3 +831,44 @@ def test_engine_over_an_8bit_pool(dtype):
     assert e1.run()[rid] == want[2]
     with pytest.raises(ValueError, match="kv_dtype"):
         Engine(m, 8, kv_dtype=torch.float16)
+
+
+# --------------------------------------------------------------------- the same bits behind tables of any width
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd,bs", [(torch.bfloat16, 32, 8, 128, 16), (torch.float32, 8, 2, 64, 16),
+                                                (torch.bfloat16, 40, 2, 256, 16), (torch.float32, 12, 12, 64, 20),
+                                                (torch.float32, 20, 2, 128, 32), (torch.bfloat16, 8, 2, 80, 8),
+                                                (torch.float32, 8, 2, 40, 16)])
+def test_decode_bits_of_short_rows_do_not_depend_on_the_table(dtype, nh, nkv, hd, bs):
+    """Rows of 1 to 512 visible slots behind a table of at most 512 (no join) and behind wider ones."""
+    lengths = [1, 2, 17, 33, 100, 257, 500, 511, 512, 0]
+    q, pools, table, positions, n_slots = decode_case(dtype, lengths, nh, nkv, hd, bs, seed=21)
+    narrow = check_decode(q, pools, table, positions, 512, nh, nkv, hd)
+    for times in (2, 9):
+        wide = torch.cat([table] + [torch.zeros_like(table)] * (times - 1), 1)
+        out = torch.full_like(q, 5.0)
+        ops.attention_decode_quant(q, ops.quant_paged_desc(*pools, wide), times * n_slots, positions, out, len(lengths),
+                                   nh, nkv, hd)
+        assert torch.equal(out, narrow), times
+    # beside a long row
+    long = torch.randint(0, pools[0].shape[0], (1, 3 * table.shape[1]), generator=gen(3), device=DEV)
+    tables = torch.cat([torch.cat([table, table, table], 1), long])
+    out = torch.empty(len(lengths) + 1, nh * hd, dtype=dtype, device=DEV)
+    ops.attention_decode_quant(torch.cat([q, q[:1]]), ops.quant_paged_desc(*pools, tables), 3 * n_slots,
+                               torch.cat([positions, positions.new_tensor([3 * n_slots - 1])]), out, len(lengths) + 1, nh,
+                               nkv, hd)
+    assert torch.equal(out[:-1], narrow)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decode_step_logits_do_not_depend_on_the_table(dtype):
+    """A model's decode step over an 8-bit pool: an eager step's table and a captured graph's, padded to max_seq_len."""
+    cfg, m = model_pair(dtype, d_model=256, n_heads=4, n_kv_heads=2, max_seq_len=2048)
+    pool = PagedKVPool(cfg, 40, 16, dtype=F8, device=DEV)
+    idx = torch.randint(0, 64, (3, 90), generator=torch.Generator().manual_seed(1))
+    pos = torch.arange(90).expand(3, 90)
+    table = torch.randperm(40, generator=torch.Generator().manual_seed(2))[:18].view(3, 6)
+    m(idx[:, :89], pos[:, :89], pool.views(table, pos[:, :89]))
+    want = m(idx[:, 89:], pos[:, 89:], pool.views(table, pos[:, 89:]))
+    wide = torch.cat([table, torch.zeros(3, 122, dtype=torch.int64)], 1)
+    assert torch.equal(m(idx[:, 89:], pos[:, 89:], pool.views(wide, pos[:, 89:])), want)
