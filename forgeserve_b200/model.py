@@ -82,11 +82,17 @@ def rope_tables(rotary_dim: int, max_len: int, theta: float, scaling: Optional[d
     return (angles.cos() * factor).float(), (angles.sin() * factor).float()
 
 
+def plain_rope(cfg: ModelConfig) -> bool:
+    """Whether cfg asks for the reference's rotary form: half layout, whole heads, positions as they are."""
+    return cfg.rope_scaling is None and cfg.rope_layout == "half" and cfg.rotary_width == cfg.head_dim
+
+
 class RopeTables:
-    """fp32 cos/sin tables per device; the kernels round them to the activation dtype as the reference does."""
+    """fp32 cos/sin tables per device. The plain form's kernel rounds them to the activation dtype, as the reference does; the
+    others take them as they are."""
 
     def __init__(self, cfg: ModelConfig):
-        if cfg.rope_scaling is None and cfg.rope_layout == "half" and cfg.rotary_width == cfg.head_dim:
+        if plain_rope(cfg):
             self.cos, self.sin = precompute_rope(cfg.head_dim, cfg.max_seq_len, cfg.rope_theta)
         else:
             self.cos, self.sin = rope_tables(cfg.rotary_width, cfg.max_seq_len, cfg.rope_theta, cfg.rope_scaling)
@@ -138,8 +144,8 @@ class Attention(nn.Module):
         self.nh, self.nkv = cfg.n_heads // tp.size, cfg.n_kv_heads // tp.size
         self.rep = cfg.n_heads // cfg.n_kv_heads
         self.rope_layout = cfg.rope_layout
-        # the reference's form (half layout, whole head) keeps its own kernel and bf16 rounding points
-        self.plain_rope = cfg.rope_layout == "half" and cfg.rotary_width == cfg.head_dim
+        # the reference's form keeps its own kernel and bf16 rounding points
+        self.plain_rope = plain_rope(cfg)
         f = dict(bias=False, device=device, dtype=dtype)
         self.wq = nn.Linear(cfg.d_model, self.nh * self.hd, **f)
         self.wk = nn.Linear(cfg.d_model, self.nkv * self.hd, **f)

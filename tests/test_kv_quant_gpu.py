@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 
 from forgeserve_b200 import _lib as L
 from forgeserve_b200 import Engine, ForgeModel, ModelConfig, PagedKVPool, generate, ops
-from forgeserve_b200.model import rope_tables
+from forgeserve_b200.model import _rope_write, rope_tables
 from oracle import forge_oracle as O
 
 DEV = "cuda"
@@ -872,3 +872,33 @@ def test_decode_step_logits_do_not_depend_on_the_table(dtype):
     want = m(idx[:, 89:], pos[:, 89:], pool.views(table, pos[:, 89:]))
     wide = torch.cat([table, torch.zeros(3, 122, dtype=torch.int64)], 1)
     assert torch.equal(m(idx[:, 89:], pos[:, 89:], pool.views(wide, pos[:, 89:])), want)
+
+
+@pytest.mark.parametrize("scaling", [{"kind": "linear", "factor": 4.0}, {"kind": "ntk", "factor": 8.0},
+                                     {"kind": "by_parts", "factor": 8.0, "original_max_len": 64, "attn_factor": 1.2}])
+def test_scaled_rotation_of_a_bf16_layer_rounds_once(scaling):
+    """Whole heads in half layout with stretched positions over a plain cache: q and the stored k against 64 bits with one
+    rounding, and q as over an 8-bit pool."""
+    cfg, m = model_pair(torch.bfloat16, d_model=512, max_seq_len=1024, rope_scaling=scaling)
+    a, hd, nh, nkv, bs = m.layers[0].attn, cfg.head_dim, cfg.n_heads, cfg.n_kv_heads, 16
+    cos, sin = m._rope.on(torch.device(DEV))
+    B, T = 2, 40
+    pos = (torch.tensor([[3], [900]]) + torch.arange(T)).to(DEV)
+    qkv = torch.randn(B * T, (nh + 2 * nkv) * hd, generator=gen(1), device=DEV).bfloat16()
+    table = torch.arange(128, device=DEV).view(2, 64)
+    qs = []
+    for dtype in (torch.bfloat16, F8):
+        pool = PagedKVPool(cfg, 128, bs, dtype=dtype, device=DEV)
+        rows = qkv.clone()
+        _rope_write(a, rows, cos, sin, pos, pool.views(table, pos)[0].descriptor(), B, T, 0, True)
+        qs.append(rows[:, : nh * hd])
+        if dtype == torch.bfloat16:
+            k = pool.k[0]
+    assert torch.equal(qs[0], qs[1])
+    p = pos.view(-1)
+    y, mag = rotate64(qkv.view(B * T, -1, hd).double()[:, : nh + nkv], cos.double()[p], sin.double()[p], "half")
+    tol = HALF[torch.bfloat16] * y.abs() + 6 * U * mag
+    assert ((qs[0].view(B * T, nh, hd).double() - y[:, :nh]).abs() <= tol[:, :nh]).all()
+    row = torch.arange(B, device=DEV).repeat_interleave(T)
+    got = k[table[row, p // bs], :, p % bs].double()
+    assert ((got - y[:, nh:]).abs() <= tol[:, nh:]).all()
