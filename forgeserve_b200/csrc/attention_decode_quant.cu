@@ -189,10 +189,13 @@ __global__ void __launch_bounds__(128) quant_decode_kernel(Params p) {
 //
 // Q enters as f16 after a scale by a power of two that brings each head's largest |q| to [1, 2): exact for bf16 down to
 // 2^-14 of it, off by 2^-25 of it below. fp32 queries enter as two halves (a value and its remainder times 2^11): 22
-// bits. P enters in f16 (2^-11) as p_j vs_j against a running maximum of its own, so that values whose scales differ
-// widely keep the f16 range: P = exp2(s + log2 vs - mo), mo >= max(s + log2 vs) - SLACK. fp32 takes log2 vs as exponent
-// and mantissa, and P's remainder as a second product. Maxima are raised only when a score exceeds them by SLACK: one
-// vote a step instead of a reduction.
+// bits. P enters in f16 (2^-11 of itself) as p_j vs_j against a running maximum of its own: P = exp2(s + log2 vs - mo),
+// max(s + log2 vs) - mo between HEADROOM and HEADROOM + SLACK, so that the largest P lies near the end of f16's range.
+// What lies 2^20 below the largest p vs of its warp's keys meets f16's smallest steps and is off by 2^-31 of that largest
+// one. fp32 takes log2 vs as exponent and mantissa and P's remainder as a second product: 22 bits, then off by 2^-37 of
+// the largest (a smaller SLACK leaves more HEADROOM: 64 rows of 2048 to 4096 slots 89.8 us against 88.3; remainders times
+// 2^11, and codes by 2^-11 beside them, would end at 2^-42 and take 97.8). The sum l of the p is fp32 throughout.
+// Maxima are raised only when a score exceeds them by SLACK: one vote a step instead of a reduction.
 //
 // 64 rows of 2176 to 4352 slots of 8 x 128 values, 32 query heads: 78 us with the join, 86 % of HBM (bf16 queries); 2
 // rows of 131072: 91 us, 92 %. The copies alone, without a product, take 68 us of the first, the join 6.
@@ -200,7 +203,7 @@ namespace tc {
 
 constexpr int WARPS = 4, TILE = 16, STEP = 32;   // a warp takes STEP keys (two tiles) at a time
 constexpr int SEG = 4;         // steps whose places a warp looks up at once
-constexpr float SLACK = 8.f, LOWEST = -3e38f;
+constexpr float LOWEST = -3e38f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -292,6 +295,9 @@ __device__ __forceinline__ void split_scale(float vs, float& e, float& mant) {
 template <typename T, int HD, int NT, bool WHOLE>
 struct Geo {
   static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;        // f16 terms of q and of p
+  // What a score may exceed its reference maximum by, and where P lies at that maximum, in powers of two: together, with a
+  // mantissa, below f16's 2^16.
+  static constexpr float SLACK = PARTS == 2 ? 2.f : 8.f, HEADROOM = 14.f - SLACK;
   static constexpr int KS = HD / 16;                          // k steps of S^T, and m tiles of O^T
   static constexpr int KC = HD / 64;                          // 16-byte chunks a lane takes of a K row
   static constexpr int VB = HD / 8 < 16 ? 8 : 16;             // bytes a lane takes of a V row at once
@@ -625,7 +631,7 @@ __device__ __forceinline__ bool decode_split(const Params& p, const CUtensorMap*
         tm[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
         tmo[n][c] = fmaxf(fmaxf(s[0][n][c] + e[0][0], s[0][n][c + 2] + e[0][1]),
                           fmaxf(s[1][n][c] + e[1][0], s[1][n][c + 2] + e[1][1]));
-        raise |= tm[n][c] > m[n][c] + SLACK || tmo[n][c] > mo[n][c] + SLACK;
+        raise |= tm[n][c] > m[n][c] + G::SLACK || tmo[n][c] > mo[n][c] + (G::HEADROOM + G::SLACK);
       }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -639,7 +645,7 @@ __device__ __forceinline__ bool decode_split(const Params& p, const CUtensorMap*
             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
           }
           x = fmaxf(x, m[n][c]);
-          y = fmaxf(y, mo[n][c]);
+          y = fmaxf(y - G::HEADROOM, mo[n][c]);
           const float co = ex2(mo[n][c] - y);
           l[n][c] *= ex2(m[n][c] - x);
 #pragma unroll

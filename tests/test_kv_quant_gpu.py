@@ -902,3 +902,96 @@ def test_scaled_rotation_of_a_bf16_layer_rounds_once(scaling):
     row = torch.arange(B, device=DEV).repeat_interleave(T)
     got = k[table[row, p // bs], :, p % bs].double()
     assert ((got - y[:, nh:]).abs() <= tol[:, nh:]).all()
+
+
+# ----------------------------------------------------------------------- small probabilities beside large ones
+
+def far_ref(q, k, v, ks, vs, table, n, nh, nkv, hd):
+    """(out, bound) of one row in 64 bits, as decode_ref, but with probabilities held to a fixed part of themselves down to
+    2^-30 (bf16) or 2^-36 (fp32) of the largest p vs. A weight in f16, and fp32's remainder of it, is off by 2^-25 where
+    f16's steps are smallest; the largest weight lies at 2^6 or above (fp32: 2^12), so that is 2^-31 (2^-37) of it, and one
+    bit for the sum that it is divided by."""
+    bs, rep, bf16 = k.shape[2], nh // nkv, q.dtype == torch.bfloat16
+    t = torch.arange(n, device=DEV)
+    blk, s = table[0][t // bs], t % bs
+    kk, vv = (c.view(torch.uint8)[blk, :, s].view(F8).double().transpose(0, 1) for c in (k, v))
+    ksr, vsr = ks[blk, :, s].double().t(), vs[blk, :, s].double().t()
+    qq = q[0].double().view(nkv, rep, hd)
+    p = torch.softmax(torch.einsum("grd,gnd->grn", qq, kk) * ksr[:, None] / math.sqrt(hd), -1)
+    vd = vv * vsr[..., None]
+    mag = torch.einsum("grd,gnd->grn", qq.abs(), kk.abs()) * ksr[:, None] / math.sqrt(hd)
+    ds = (hd + 8) * U * mag.amax(-1)
+    qerr = qq.abs().amax(-1) * 2.0 ** -25 * (kk.abs().sum(-1) * ksr).amax(-1)[:, None] / math.sqrt(hd) if bf16 else 0
+    rel = 2 * (ds + qerr) + (2.0 ** -11 + 2.0 ** -12 if bf16 else 2.0 ** -21) + (n + 64) * U
+    floor = (p * vsr[:, None]).amax(-1) * 2.0 ** (-30 if bf16 else -36) * vv.abs().sum(1).amax(-1)[:, None]
+    out = torch.einsum("grn,gnd->grd", p, vd)
+    bound = torch.einsum("grn,gnd->grd", p, vd.abs()) * rel[..., None] + floor[..., None]
+    return out.reshape(1, -1), bound.reshape(1, -1)
+
+
+def far_check(dtype, q, pools, table, n, nh, nkv, hd):
+    out = torch.empty_like(q)
+    ops.attention_decode_quant(q, ops.quant_paged_desc(*pools, table), n, torch.tensor([n - 1], device=DEV), out, 1, nh, nkv,
+                               hd)
+    want, bound = far_ref(q, *pools, table, n, nh, nkv, hd)
+    tol = HALF[dtype] * (want.abs() + bound) + bound
+    worst = ((out.double() - want).abs() / tol).max().item()
+    assert worst <= 1, worst
+
+
+FAR = [(torch.bfloat16, 8, 2, 128, 16), (torch.bfloat16, 8, 2, 64, 20), (torch.float32, 8, 2, 64, 16),
+       (torch.float32, 4, 4, 128, 20), (torch.float32, 20, 2, 64, 16), (torch.bfloat16, 24, 2, 256, 16),
+       (torch.float32, 4, 2, 256, 16), (torch.float32, 8, 2, 40, 16)]
+
+
+@pytest.mark.parametrize("gap", [0, 14, 20, 25, 30])
+@pytest.mark.parametrize("dtype,nh,nkv,hd,bs", FAR)
+def test_decode_of_one_key_far_above_the_others(dtype, nh, nkv, hd, bs, gap):
+    """A key 2^gap above 499 others, whose value is zero in half of the dims: there the others make the whole output."""
+    n = 500
+    q, pools, table, _, _ = decode_case(dtype, [n], nh, nkv, hd, bs, seed=31)
+    k, v, ks, vs = pools
+    ks.fill_(1.0)
+    vs.fill_(1.0)
+    codes = torch.zeros(k.shape, device=DEV)
+    b, s = table[0, 70 // bs], 70 % bs
+    codes[b, :, s, 0] = 1.0
+    k.copy_(codes.to(F8))
+    v.view(torch.uint8)[b, :, s, hd // 2:] = 0
+    q.zero_().view(1, nh, hd)[:, :, 0] = gap * math.sqrt(hd) * math.log(2)
+    far_check(dtype, q, pools, table, n, nh, nkv, hd)
+
+
+@pytest.mark.parametrize("apart", [12, 20, 26])
+@pytest.mark.parametrize("dtype,nh,nkv,hd,bs", FAR)
+def test_decode_of_values_whose_scales_lie_far_apart(dtype, nh, nkv, hd, bs, apart):
+    """Every other key's value 2^apart below its neighbours', in dims where those have zeros."""
+    n = 500
+    q, pools, table, _, _ = decode_case(dtype, [n], nh, nkv, hd, bs, seed=32)
+    k, v, ks, vs = pools
+    vs.fill_(1.0)
+    t = torch.arange(n, device=DEV)
+    b, s = table[0][t // bs], t % bs
+    low = t % 2 == 1
+    vs[b[low], :, s[low]] = 2.0 ** -apart
+    raw = v.view(torch.uint8)
+    raw[b[low], :, s[low], : hd // 2] = 0
+    raw[b[~low], :, s[~low], hd // 2:] = 0
+    far_check(dtype, q, pools, table, n, nh, nkv, hd)
+
+
+def test_decode_of_one_key_far_above_a_long_row():
+    """32 KV heads, 50000 keys 2^25 below one of them: a warp holds 768 keys of a split."""
+    n, nh, nkv, hd, bs = 50000, 32, 32, 64, 64
+    q, pools, table, _, _ = decode_case(torch.float32, [n], nh, nkv, hd, bs, seed=33)
+    k, v, ks, vs = pools
+    ks.fill_(1.0)
+    vs.fill_(1.0)
+    codes = torch.zeros(k.shape, device=DEV)
+    b, s = table[0, 33000 // bs], 33000 % bs
+    codes[b, :, s, 0] = 1.0
+    k.copy_(codes.to(F8))
+    v.view(torch.uint8)[:] &= 0x7F                                  # of one sign: lost ones are missed
+    v.view(torch.uint8)[b, :, s, hd // 2:] = 0
+    q.zero_().view(1, nh, hd)[:, :, 0] = 25 * math.sqrt(hd) * math.log(2)
+    far_check(torch.float32, q, pools, table, n, nh, nkv, hd)
