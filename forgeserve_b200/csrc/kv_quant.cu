@@ -8,7 +8,8 @@
 // intermediate roundings would have to be kept (rope_kv_kernel in elementwise.cu keeps them for the plain form).
 //
 // 8-bit cache: a (slot, KV head) row of hd values has one fp32 scale = max(max|x| / 448, 2^-126) and hd codes
-// e4m3(x / scale), rounded to nearest even; 448 is e4m3's largest value, and the floor on the scale keeps 1 / scale
+// e4m3(x r), rounded to nearest even, with r = 1 / scale to 2^-22: the codes of x / scale, but where that lies within 2^-21
+// of itself of a border between two codes either one. 448 is e4m3's largest value, and the floor on the scale keeps 1 / scale
 // finite (a row of zeros gets zero codes). A row holding an infinity or a NaN gets an infinite or NaN scale and reads
 // back as NaN. A scale for each row costs 4 bytes on hd and needs no calibration, and a row can be written without
 // reading its block. Codes lie as the values of an unquantised cache do; scales as (num_blocks, n_kv, block_size).

@@ -193,8 +193,9 @@ typedef struct {
  * call must not share a slot: which of them a shared slot then holds, or in what mixture, is not defined.
  *   fs_rotary_kv_write: the cache holds values of `dtype`.
  *   fs_rotary_kv_write_quant: the cache holds codes. Each (token, KV head) row of k and of v gets the scale
- *     max(max|x| / 448, 2^-126) and the codes e4m3(x / scale), nearest even; a row with an infinity or a NaN reads back
- *     as NaN. */
+ *     max(max|x| / 448, 2^-126), off by 2^-23 of itself at most, and the codes e4m3(x / scale), nearest even (either of two
+ *     codes where x / scale lies within 2^-21 of itself of their border: x is multiplied by an approximate 1 / scale); a
+ *     row with an infinity or a NaN reads back as NaN. */
 int fs_rotary_kv_write(const void* qkv, int64_t ld, void* q_out, int64_t ldq, const float* cos_t, const float* sin_t,
                        int64_t rope_rows, int64_t rotary_dim, int interleaved, const int64_t* positions,
                        const fs_kv_cache* kv, int64_t B, int64_t T, int64_t nh, int64_t nkv, int64_t hd,

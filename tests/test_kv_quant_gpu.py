@@ -8,6 +8,7 @@ import subprocess
 import sys
 from pathlib import Path
 
+import numpy as np
 import pytest
 import torch
 
@@ -995,3 +996,42 @@ def test_decode_of_one_key_far_above_a_long_row():
     v.view(torch.uint8)[b, :, s, hd // 2:] = 0
     q.zero_().view(1, nh, hd)[:, :, 0] = 25 * math.sqrt(hd) * math.log(2)
     far_check(torch.float32, q, pools, table, n, nh, nkv, hd)
+
+
+@pytest.mark.parametrize("hd", [128, 64, 80, 18])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_store_codes_beside_borders(dtype, hd):
+    """The documented bounds: scales off by 2^-23 of top / 448, and codes those of x / scale or, where that lies within
+    2^-21 of itself of a border between two codes, one of the two; over random rows and rows of values at and beside the
+    borders. (1 / scale is off by 2 steps of 2^-23, its product with x by 2^-24: less than 2^-21.)"""
+    T, nkv, bs = 400, 2, 16
+    rows = torch.randn(T, 2 * nkv, hd, generator=gen(1), device=DEV) * torch.exp(
+        3 * torch.randn(T, 2 * nkv, 1, generator=gen(2), device=DEV))
+    steps = torch.arange(256, dtype=torch.uint8)
+    values = steps.view(F8).float()
+    values = values[torch.isfinite(values) & (steps < 128)]
+    borders = ((values[1:] + values[:-1]) / 2).to(DEV)
+    for r in range(0, T, 2):
+        scale = 2.0 ** (r % 37 - 18) * (1 + (r * 0.37) % 1)
+        pick = borders[torch.randint(0, borders.numel(), (2 * nkv, hd), generator=gen(r), device=DEV)] * scale
+        up = torch.randint(-2, 3, pick.shape, generator=gen(r + 1), device=DEV)
+        rows[r] = (pick.view(torch.int32) + up.int()).view(torch.float32)
+        rows[r, :, 0] = 448 * scale
+    x = rows.to(dtype)
+    pools = quant_pool(T // bs + 1, nkv, bs, hd, 1)
+    table = torch.randperm(T // bs + 1, generator=gen(4), device=DEV)[: T // bs][None]
+    ops.rotary_kv_write(x.view(T, -1), None, None, torch.arange(T, device=DEV), ops.quant_paged_desc(*pools, table), 1, T, 0,
+                        nkv, hd)
+    t = torch.arange(T, device=DEV)
+    for i, part in enumerate((x[:, :nkv], x[:, nkv:])):
+        part = part.double().cpu()
+        top = part.abs().amax(-1) / 448
+        scale = pools[2 + i][table[0, t // bs], :, t % bs].cpu().double()
+        assert ((scale - top).abs() <= 2.0 ** -23 * top).all()
+        z = (part / scale[..., None]).abs().numpy()
+        near, far = (torch.from_numpy((z * (1 + e)).astype(np.float32)).to(F8).float() for e in (-(2.0 ** -21), 2.0 ** -21))
+        raw = bits(pools[i]).view(pools[i].shape)[table[0, t // bs], :, t % bs].cpu()
+        got = raw.view(F8).float()
+        assert ((near <= got.abs()) & (got.abs() <= far)).all()
+        assert torch.equal(raw >= 128, torch.signbit(part))
+        assert (near != far).any() or hd == 18
