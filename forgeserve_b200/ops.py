@@ -436,6 +436,15 @@ def paged_desc(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> L.KVCac
     return desc
 
 
+def _strides(t: torch.Tensor) -> tuple:
+    """t's strides, those of dimensions of one entry (which address nothing) as if t were contiguous from there on."""
+    out, step = [], 1
+    for n, st in zip(reversed(t.shape), reversed(t.stride())):
+        out.append(step if n == 1 else st)
+        step *= n
+    return tuple(reversed(out))
+
+
 _PACK_QUANT = struct.Struct("13q").pack   # the fields of KVQuantDesc, all 8 bytes
 
 
@@ -453,11 +462,13 @@ def quant_paged_desc(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_
     rows = (nblk, nkv, bs)
     if v.shape != shape or k_scale.shape != rows or v_scale.shape != rows:
         raise ValueError("quant_paged_desc: k, v and their scales must describe one pool")
-    s0, s1, s2, s3 = strides = k.stride()
-    c0, c1, c2 = cols = k_scale.stride()
-    if (v.stride() != strides or v_scale.stride() != cols or s3 != 1 or s2 != hd or c2 != 1
-            or s0 < 0 or s1 < 0 or c0 < 0 or c1 < 0):
-        raise ValueError("quant_paged_desc: the slots of a (block, head) must lie contiguously, k and v alike")
+    strides, cols = k.stride(), k_scale.stride()
+    if v.stride() != strides or v_scale.stride() != cols or strides[2:] != (hd, 1) or cols[2] != 1:
+        strides, cols = _strides(k), _strides(k_scale)   # apart from the dimensions of one entry
+        if _strides(v) != strides or _strides(v_scale) != cols or strides[2:] != (hd, 1) or cols[2] != 1:
+            raise ValueError("quant_paged_desc: the slots of a (block, head) must lie contiguously, k and v alike")
+    s0, s1, _, _ = strides
+    c0, c1, _ = cols
     (n, width), (t0, t1) = table.shape, table.stride()
     if table.dtype != torch.int64 or t1 != 1 and width > 1:
         raise ValueError("the block table must be int64 with contiguous rows")

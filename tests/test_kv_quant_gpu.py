@@ -1035,3 +1035,19 @@ def test_store_codes_beside_borders(dtype, hd):
         assert ((near <= got.abs()) & (got.abs() <= far)).all()
         assert torch.equal(raw >= 128, torch.signbit(part))
         assert (near != far).any() or hd == 18
+
+
+def test_pool_of_one_block_cut_from_a_larger_one():
+    """k and its scales cut from a larger pool, v and its own: strides that differ in dimensions of one entry alone."""
+    for nkv, bs in ((3, 32), (1, 1)):
+        k, v, ks, vs = quant_pool(5, nkv + 1, bs, 64, 41)
+        cut = [p[2:3, :nkv] for p in (k, v, ks, vs)]
+        mixed = [cut[0], cut[1].contiguous(), cut[2], cut[3].contiguous()] if nkv == 1 else cut
+        q = torch.randn(2, 2 * nkv * 64, generator=gen(42), device=DEV).bfloat16()
+        table, n = torch.zeros(2, 1, dtype=torch.int64, device=DEV), bs
+        pos = torch.tensor([n - 1, 0], device=DEV)
+        got = check_decode(q, mixed, table, pos, n, 2 * nkv, nkv, 64)
+        assert torch.equal(got, check_decode(q, [c.contiguous() for c in cut], table, pos, n, 2 * nkv, nkv, 64))
+        kd, vd = ops.kv_dequant(ops.quant_paged_desc(*mixed, table), 2, n, nkv, 64, torch.float32)
+        for d, c, s in ((kd, cut[0], cut[2]), (vd, cut[1], cut[3])):
+            assert torch.equal(d[0], (c.float() * s[..., None])[0])

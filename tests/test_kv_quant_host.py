@@ -180,3 +180,27 @@ def test_dequant_and_decode_refusals(lib):
     for kw in (dict(), dict(ws=P, wsb=need - 1), dict(ws=ctypes.c_void_p(4097), wsb=need)):
         assert dec(kv=ctypes.byref(long), n=1024, **kw) == -1 and b"workspace" in lib.fs_last_error()
     assert dec(B=0) == 0
+
+
+def test_descriptor_takes_strides_of_single_entries_as_they_come():
+    """A dimension of one entry has no stride that matters: slices that differ there alone are one pool."""
+    k = torch.zeros(4, 2, 8, 16).to(F8)
+    s, t = torch.zeros(4, 2, 8), torch.zeros(1, 2, dtype=torch.int64)
+    # one KV head, one slot a block, one block; v and the scales with memory of their own
+    for cut in ((slice(None), slice(1, 2)), (slice(None), slice(None), slice(0, 1)), (slice(3, 4),),
+                (slice(0, 1), slice(0, 1)), (slice(0, 1), slice(0, 1), slice(5, 6))):
+        kc, sc = k[cut], s[cut]
+        d = ops.quant_paged_desc(kc, kc.clone(memory_format=torch.contiguous_format), sc, sc.contiguous(), t) \
+            if kc.shape[0] == 1 else ops.quant_paged_desc(kc, kc, sc, sc, t)
+        assert d.cache.k == kc.data_ptr() and d.k_scale == sc.data_ptr()
+        assert (d.cache.block_size, d.cache.num_blocks) == (kc.shape[2], kc.shape[0])
+        assert d.cache.block_stride >= 0 and d.cache.block_stride % 16 == 0 and d.cache.head_stride % 16 == 0
+    spread = s[:, :, ::8]                                            # one slot a block, slots eight apart
+    assert spread.stride(2) == 8
+    d = ops.quant_paged_desc(k[:, :, :1], k[:, :, :1], spread, spread, t)
+    assert (d.scale_block_stride, d.scale_head_stride) == (16, 8)
+    d = ops.quant_paged_desc(k[:, :1], k[:, :1], s[:, :1], s[:, :1], t)
+    assert d.cache.block_stride == 256 and d.scale_block_stride == 16
+    for args in ((k, torch.zeros(4, 4, 8, 16).to(F8)[:, :2], s, s, t), (k, k, s, torch.zeros(4, 4, 8)[:, :2], t)):
+        with pytest.raises(ValueError, match="alike"):               # more than one entry: the strides have to agree
+            ops.quant_paged_desc(*args)
