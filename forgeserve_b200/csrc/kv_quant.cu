@@ -354,6 +354,10 @@ struct Lane {
 // token's items each time (whole warps of them, so that a warp's stay alike): heads for the cache cost more than heads of
 // q, and where the grid is a multiple of a token's items every warp would meet the same heads again and again (16 x 2048
 // tokens of 32 + 8 + 8 heads: 152 us instead of 116).
+// A lane without items stands at `count` and is moved on as often as the others of its warp: to less than twice the count
+// and two steps, which has to stay within 32 bits.
+constexpr int64_t MOST_ITEMS = (int64_t{1} << 31) - (1 << 20), MOST_STEP = 148 * WRITE_CTAS * 256;
+static_assert(2 * (MOST_ITEMS + MOST_STEP) <= int64_t{1} << 32, "item numbers would wrap");
 struct Items {
   unsigned count, groups, step, step_tok, step_group, item, token, group;
   __device__ __forceinline__ Items(const WriteParams& p, int lanes, unsigned n_groups) {
@@ -617,8 +621,8 @@ int write_t(const WriteParams& p, bool quant, int interleaved, cudaStream_t st) 
   constexpr int PIECES = 32 / static_cast<int>(sizeof(T));   // values a lane of the vector form holds of a head
   int lanes = 1;
   while (lanes * PIECES < p.hd) lanes *= 2;
-  const int64_t vec_items = p.tokens * ((p.nh + 2 * p.nkv + 1) / 2) * lanes;   // thread numbers of 31 bits
-  if (write_vec_ok<T>(p, quant) && vec_items <= INT32_MAX) {
+  const int64_t vec_items = p.tokens * ((p.nh + 2 * p.nkv + 1) / 2) * lanes;   // thread numbers
+  if (write_vec_ok<T>(p, quant) && vec_items <= MOST_ITEMS) {
     const unsigned groups = (p.nh + 2 * p.nkv + WRITE_HEADS - 1) / WRITE_HEADS;
     const int64_t blocks = (p.tokens * groups * lanes + 255) / 256;
     auto launch = [&](auto kernel, int ctas) {
