@@ -1051,3 +1051,125 @@ def test_pool_of_one_block_cut_from_a_larger_one():
         kd, vd = ops.kv_dequant(ops.quant_paged_desc(*mixed, table), 2, n, nkv, 64, torch.float32)
         for d, c, s in ((kd, cut[0], cut[2]), (vd, cut[1], cut[3])):
             assert torch.equal(d[0], (c.float() * s[..., None])[0])
+
+
+def test_model_over_an_8bit_pool_stays_near_the_quantised_model():
+    """fp32: a code moves one step where rounding errors of some 2^-20 cross a border, one value in some 10^4, which makes
+    about a hundredth of the quantisation's own distance; a quarter of that distance is allowed. bf16: whatever its own
+    roundings do, the logits lie nearer to the model with a quantised cache than to the one without."""
+    for dtype, kw in ((torch.float32, {}), (torch.float32, dict(rope_layout="interleaved", rotary_dim=6)),
+                      (torch.float32, dict(rope_scaling={"kind": "ntk", "factor": 4.0})),
+                      (torch.bfloat16, dict(d_model=512)), (torch.bfloat16, dict(d_model=256, n_kv_heads=4))):
+        cfg, m = model_pair(dtype, **kw)
+        idx = torch.randint(0, 64, (2, 30), generator=torch.Generator().manual_seed(1))
+        plain, want = logits64(m, cfg, idx), logits64(m, cfg, idx, fake_quant=True)
+        pool = PagedKVPool(cfg, 20, 4, dtype=F8, device=DEV)
+        table = torch.randperm(20, generator=torch.Generator().manual_seed(2))[:16].view(2, 8)
+        pos = torch.arange(30).expand(2, 30)
+        got = [m(idx[:, a:b], pos[:, a:b], pool.views(table, pos[:, a:b]))
+               for a, b in [(0, 17), (17, 26)] + [(i, i + 1) for i in range(26, 30)]]
+        got = torch.cat(got, 1).double().cpu()
+        if dtype == torch.float32:
+            assert (got - want).norm() <= 0.25 * (plain - want).norm(), kw
+        else:
+            assert (got - want).norm() < (got - plain).norm(), kw
+
+
+REQUESTS = [([(7 * i + j) % 64 for j in range(3 + 5 * i)], 20) for i in range(4)]
+
+
+def test_engine_preempts_over_an_8bit_pool():
+    """A pool too small for its requests (fp32): blocks are taken back and used again with old codes and scales in them, and
+    the tokens are those of a large pool. Each token is the best of a prefill of what came before over a fresh 8-bit
+    pool, or within 2^-6 of the logits' spread of it (codes beside a border may differ)."""
+    cfg, m = model_pair(torch.float32, d_model=256, n_heads=4, n_kv_heads=2)
+
+    def run(blocks, **kw):
+        e = Engine(m, num_blocks=blocks, block_size=4, max_batch=4, kv_dtype=F8, **kw)
+        ids = [e.add_request(p, n) for p, n in REQUESTS]
+        out = e.run()
+        assert e.pool.allocator.num_free == blocks
+        return [out[i] for i in ids], e.preemptions
+
+    want, none = run(64, cuda_graphs=False)
+    assert none == 0
+    for kw in (dict(cuda_graphs=False), dict()):
+        got, some = run(14, **kw)
+        assert some > 0 and got == want, kw
+    for (prompt, n), out in zip(REQUESTS, want):
+        assert len(out) == n
+        seq = prompt + out
+        pool = PagedKVPool(cfg, 16, 4, dtype=F8, device=DEV)
+        pos = torch.arange(len(seq))[None]
+        logits = m(torch.tensor([seq]), pos, pool.views(torch.arange(-(-len(seq) // 4))[None], pos))[0]
+        logits = logits[len(prompt) - 1: -1].double()
+        spread = logits.amax(-1) - logits.amin(-1)
+        chosen = logits.gather(1, torch.tensor(out, device=DEV)[:, None])[:, 0]
+        assert (chosen >= logits.amax(-1) - 2.0 ** -6 * spread).all()
+
+
+def pipeline_8bit_worker(rank, size, cfg_dict, sd, blocks, microbatches, pieces):
+    from forgeserve_b200 import PipelineEngine, PipelineStage
+    stage = PipelineStage(ModelConfig(**cfg_dict), rank, size)
+    stage.load_from_full(sd)
+    eng = PipelineEngine(stage.eval(), num_blocks=blocks, block_size=4, max_batch=4, microbatches=microbatches,
+                         prefill_chunks=pieces, kv_dtype=F8)
+    assert eng.pool.quantized and len(eng.pool.k) == len(stage.layers)
+    ids = [eng.add_request(p, n) for p, n in REQUESTS]
+    out = eng.run()
+    return [out[i] for i in ids], eng.preemptions, eng.pool.allocator.num_free
+
+
+@pytest.mark.parametrize("size,microbatches,pieces,blocks", [(2, 1, 1, 64), (2, 2, 1, 14), (3, 2, 3, 64)])
+def test_pipeline_engine_over_8bit_pools(size, microbatches, pieces, blocks):
+    """fp32 stages over 8-bit pools of their own layers give the Engine's tokens: prompts whole and in pieces, with
+    preemption, in micro-batches."""
+    from forgeserve_b200.tensor_parallel import run_in_threads
+    cfg, m = model_pair(torch.float32, d_model=256, n_layers=3, n_heads=4, n_kv_heads=2)
+    e = Engine(m, num_blocks=64, block_size=4, max_batch=4, kv_dtype=F8)
+    ids = [e.add_request(p, n) for p, n in REQUESTS]
+    out = e.run()
+    sd = {k: t.detach().cpu() for k, t in m.state_dict().items()}
+    for got, preemptions, free in run_in_threads(pipeline_8bit_worker, size, cfg.to_dict(), sd, blocks, microbatches, pieces):
+        assert got == [out[i] for i in ids] and free == blocks
+        assert (preemptions > 0) == (blocks == 14)
+
+
+def stage_graph_worker(rank, size, cfg_dict, sd):
+    from forgeserve_b200 import PipelineStage
+    from forgeserve_b200.pipeline_engine import _StageDecodeGraph
+    cfg = ModelConfig(**cfg_dict)
+    stage = PipelineStage(cfg, rank, size)
+    stage.load_from_full(sd)
+    stage = stage.to(torch.bfloat16).eval()
+    table = torch.randperm(16, generator=torch.Generator().manual_seed(2))[:12].view(3, 4)
+    pos = torch.arange(60).expand(3, 60)
+    idx = torch.randint(0, 64, (3, 60), generator=torch.Generator().manual_seed(1)).to(DEV)
+    got = []
+    for graph in (False, True):
+        pool = PagedKVPool(cfg, 16, 16, dtype=F8, device=DEV)
+        views = pool.views(table, pos[:, :50])
+        stage.run_layers_(stage.embed(idx[:, :50]), views[0].positions, views)
+        g = _StageDecodeGraph(stage, pool, 3) if graph else None
+        tokens = []
+        for t in range(50, 60):
+            if graph:
+                tokens.append(g.run(pos[:, t: t + 1].to(DEV), table.to(DEV), idx[:, t]).clone())
+            else:
+                views = pool.views(table, pos[:, t: t + 1])
+                x = stage.embed(idx[:, t: t + 1])
+                stage.run_layers_(x, views[0].positions, views)
+                tokens.append(ops.argmax(stage.head(x[:, -1:])[:, -1]))
+        got.append((torch.stack(tokens), *[bits(t) for t in pool.k + pool.v + pool.k_scale + pool.v_scale]))
+    torch.cuda.synchronize()
+    return all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@torch.no_grad()
+def test_stage_decode_graph_over_an_8bit_pool():
+    """A stage's captured decode step, as decode windows replay it (its table padded to max_seq_len), gives the eager
+    step's tokens and cache bit for bit."""
+    from forgeserve_b200.tensor_parallel import run_in_threads
+    cfg, m = model_pair(torch.float32, d_model=256, n_heads=4, n_kv_heads=2, max_seq_len=1024)
+    sd = {k: t.detach().cpu() for k, t in m.state_dict().items()}
+    assert run_in_threads(stage_graph_worker, 1, cfg.to_dict(), sd) == [True]
