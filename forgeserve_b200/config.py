@@ -1,7 +1,9 @@
 """Model hyper-parameters, with the reference's constructor, defaults and validation (forgeserve/config.py:7-39), and
 the rotary forms that the reference lacks (rope_layout, rotary_dim, rope_scaling)."""
 
+import math
 from dataclasses import asdict, dataclass
+from numbers import Integral, Real
 from typing import Optional
 
 _SCALING_KEYS = {"linear": {"factor"}, "ntk": {"factor"},
@@ -14,11 +16,15 @@ def check_rope_scaling(scaling: Optional[dict]) -> None:
     if not isinstance(scaling, dict):
         raise ValueError("rope_scaling must be a dict with a kind and a factor")
     kind = scaling.get("kind")
-    if kind not in _SCALING_KEYS:
+    if not isinstance(kind, str) or kind not in _SCALING_KEYS:
         raise ValueError(f"rope_scaling kind must be one of {sorted(_SCALING_KEYS)}, not {kind!r}")
     extra = set(scaling) - _SCALING_KEYS[kind] - {"kind"}
     if extra:
         raise ValueError(f"rope_scaling kind {kind!r} does not take {sorted(extra)}")
+    for name in set(scaling) - {"kind"}:
+        value = scaling[name]
+        if isinstance(value, bool) or not isinstance(value, Real) or not math.isfinite(value):
+            raise ValueError(f"rope_scaling {name} must be a finite number, not {value!r}")
     if not scaling.get("factor", 0) >= 1:
         raise ValueError("rope_scaling needs a factor of at least 1")
     if kind == "by_parts":
@@ -57,8 +63,9 @@ class ModelConfig:
             raise ValueError("head_dim must be even for rotary embeddings")
         if self.rope_layout not in ("half", "interleaved"):
             raise ValueError(f"rope_layout must be 'half' or 'interleaved', not {self.rope_layout!r}")
-        if self.rotary_dim is not None and not (0 < self.rotary_dim <= self.head_dim and self.rotary_dim % 2 == 0):
-            raise ValueError(f"rotary_dim must be even and in 2..{self.head_dim}")
+        r = self.rotary_dim
+        if r is not None and not (isinstance(r, Integral) and not isinstance(r, bool) and 0 < r <= self.head_dim and r % 2 == 0):
+            raise ValueError(f"rotary_dim must be an even whole number in 2..{self.head_dim}")
         check_rope_scaling(self.rope_scaling)
 
     @property

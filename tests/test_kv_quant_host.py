@@ -204,3 +204,28 @@ def test_descriptor_takes_strides_of_single_entries_as_they_come():
     for args in ((k, torch.zeros(4, 4, 8, 16).to(F8)[:, :2], s, s, t), (k, k, s, torch.zeros(4, 4, 8)[:, :2], t)):
         with pytest.raises(ValueError, match="alike"):               # more than one entry: the strides have to agree
             ops.quant_paged_desc(*args)
+
+
+@pytest.mark.parametrize("bad", [dict(factor=math.inf), dict(factor=math.nan), dict(factor="8"), dict(factor=None),
+                                 dict(factor=[2.0]), dict(original_max_len=math.inf), dict(original_max_len="64"),
+                                 dict(beta_fast=math.inf), dict(beta_fast=math.nan), dict(beta_slow="1"),
+                                 dict(attn_factor=math.inf), dict(attn_factor=math.nan), dict(attn_factor=None)])
+def test_config_refuses_rotary_numbers_that_are_none(bad):
+    """Anything but finite numbers in rope_scaling is a ValueError when the model is described, not tables of zeros or
+    NaN, or a TypeError, later."""
+    scaling = {"kind": "by_parts", "factor": 2, "original_max_len": 64}
+    ModelConfig(rope_scaling=scaling)
+    with pytest.raises(ValueError, match="rope_scaling"):
+        ModelConfig(rope_scaling={**scaling, **bad})
+    with pytest.raises(ValueError, match="kind"):
+        ModelConfig(rope_scaling={"kind": ["linear"], "factor": 2})
+    if "factor" in bad:
+        for kind in ("linear", "ntk"):
+            with pytest.raises(ValueError, match="rope_scaling"):
+                ModelConfig(rope_scaling={"kind": kind, **bad})
+
+
+def test_config_refuses_rotary_dims_that_are_no_whole_numbers():
+    for bad in (8.0, "8", True):
+        with pytest.raises(ValueError, match="rotary_dim"):
+            ModelConfig(rotary_dim=bad)
