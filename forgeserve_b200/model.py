@@ -229,8 +229,8 @@ def layer_forward_(blk: "Block", x: torch.Tensor, positions: torch.Tensor, kv, r
         _rope_write(a, qkv2, rope_cos, rope_sin, positions, desc, B, T, slot_base=base, slot_from_pos=from_pos)
     quant = isinstance(desc, L.KVQuantDesc)
     if quant and T > 1:
-        # several new tokens a row over an 8-bit cache: attention over the visible slots read back as dense tensors
-        k_all, v_all = ops.kv_dequant(desc, B, n_slots, nkv, hd, x.dtype)
+        # several new tokens a row over an 8-bit cache: attention over the table's slots read back as dense tensors
+        k_all, v_all = ops.kv_dequant(kv.read_descriptor(), B, n_slots, nkv, hd, x.dtype)
         table = row_table(B, x.device)
         desc, keep = ops.contiguous_desc(k_all, v_all, table), (keep, k_all, v_all, table)
     attn = torch.empty(B, T, nh * hd, dtype=x.dtype, device=x.device)

@@ -1173,3 +1173,26 @@ def test_stage_decode_graph_over_an_8bit_pool():
     cfg, m = model_pair(torch.float32, d_model=256, n_heads=4, n_kv_heads=2, max_seq_len=1024)
     sd = {k: t.detach().cpu() for k, t in m.state_dict().items()}
     assert run_in_threads(stage_graph_worker, 1, cfg.to_dict(), sd) == [True]
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 16), (torch.bfloat16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("kind", ["plain", "8-bit"])
+def test_tables_padded_with_no_block(kind, dtype, hd):
+    """Columns past a row's last token may hold anything, -1 or a number past the pool, in a prompt, a continued chunk
+    and a decode step: the same logits as with block 0 there, and nothing is flagged (the fixture looks)."""
+    cfg, m = model_pair(dtype, d_model=4 * hd, max_seq_len=512)
+    idx = torch.randint(0, 64, (2, 100), generator=torch.Generator().manual_seed(1))
+    pos = torch.arange(100).expand(2, 100)
+    blocks = torch.randperm(20, generator=torch.Generator().manual_seed(2))[:14].view(2, 7)
+    got = []
+    for pad in (0, -1, 1 << 40):
+        pool = PagedKVPool(cfg, 20, 16, dtype=F8 if kind == "8-bit" else dtype, device=DEV)
+        table = torch.cat([blocks, torch.full((2, 20), pad)], 1)
+        logits = []
+        for a, b in ((0, 70), (70, 99), (99, 100)):
+            t = table.clone()
+            t[:, -(-b // 16):] = pad                                # blocks not granted yet
+            logits.append(m(idx[:, a:b], pos[:, a:b], pool.views(t, pos[:, a:b])))
+        got.append(torch.cat(logits, 1))
+        assert L.device_error() == 0, pad
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
