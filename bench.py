@@ -351,6 +351,14 @@ C4_WORKLOAD = ("C4: 8B-shape continuous-batching decode over a paged KV cache (b
                "tokens each, one pipeline stage per GPU")
 
 
+KV_DTYPES = {"model": None, "e4m3": torch.float8_e4m3fn}
+
+
+def kv_row_bytes(head_dim: int, kv_dtype: str) -> int:
+    """Bytes of a (slot, KV head) row of keys or values: bf16, or e4m3 codes and an fp32 scale."""
+    return head_dim + 4 if kv_dtype == "e4m3" else 2 * head_dim
+
+
 def run_c4(args):
     """Config 4 through the Engine (1 GPU) or PipelineEngine (one stage per GPU): one step is the whole batch of
     64 requests from submission to the last token. Reports generated tokens/s over the run and over the decode
@@ -375,14 +383,15 @@ def run_c4(args):
         model = ForgeModel(cfg, device=dev, dtype=torch.bfloat16).eval()
         init_model_(model, seed=1234, std=0.02)
         engine = Engine(model, C4["num_blocks"], C4["block_size"], max_batch=C4["requests"], seed=0,
-                        cuda_graphs=not args.no_graphs)
+                        cuda_graphs=not args.no_graphs, kv_dtype=KV_DTYPES[args.kv_dtype])
         weight_bytes = sum(p.numel() * p.element_size() for p in model.parameters())
     else:
         stage = PipelineStage(cfg, rank, world, device=dev, dtype=torch.bfloat16).eval()
         init_stage_(stage, seed=1234, std=0.02)
         engine = PipelineEngine(stage, C4["num_blocks"], C4["block_size"], max_batch=C4["requests"], seed=0,
                                 microbatches=args.microbatches or world, overlap=False if args.no_windows else None,
-                                prefill_chunks=args.seq_chunks, cuda_graphs=not args.no_graphs)
+                                prefill_chunks=args.seq_chunks, cuda_graphs=not args.no_graphs,
+                                kv_dtype=KV_DTYPES[args.kv_dtype])
         weight_bytes = sum(p.numel() * p.element_size() for p in stage.parameters())
     rng = random.Random(11)
     lengths = [rng.randint(C4["prompt_lo"], C4["prompt_hi"]) for _ in range(C4["requests"])]
@@ -443,7 +452,7 @@ def run_c4(args):
         dec_tokens = n_req * (n_new - 1) * args.steps
         # bytes a decode step must move: every weight once (all stages) and the K/V of every cached token of
         # every layer; the mean context over the decode phase is prompt + half the generated tokens
-        kv_token = cfg.n_layers * cfg.n_kv_heads * cfg.head_dim * 2 * 2
+        kv_token = cfg.n_layers * cfg.n_kv_heads * 2 * kv_row_bytes(cfg.head_dim, args.kv_dtype)
         mean_ctx = sum(lengths) / n_req + n_new / 2
         step_bytes = weight_bytes + n_req * mean_ctx * kv_token
         step_ms = dec_ms / max(steps_dec, 1)
@@ -451,7 +460,8 @@ def run_c4(args):
             if (ROOT / "MEASURED_PEAKS.json").exists() else (6650.0, "fallback")
         achieved = step_bytes / (step_ms / 1e3) / 1e9
         result = {
-            "metric": "continuous-batching decode tokens/s, 8B-shape bf16 (config 4)",
+            "metric": "continuous-batching decode tokens/s, 8B-shape bf16 (config 4)"
+                      + (", 8-bit KV cache" if args.kv_dtype == "e4m3" else ""),
             "value": round(generated / (total_ms / 1e3), 1), "unit": "tokens/s", "n_gpus": world,
             "steps": args.steps, "warmup": max(args.warmup, 1), "ms_per_step": round(total_ms / args.steps, 1),
             "higher_is_better": True, "scaling": "strong", "vs_baseline": None, "dtype": "bf16",
@@ -459,7 +469,7 @@ def run_c4(args):
             "config": {"workload": C4_WORKLOAD, "stages": world, "parallelism": f"pp{world}",
                        "microbatches": 1 if world == 1 else (args.microbatches or world),
                        "decode_cuda_graphs": (not args.no_graphs) and (world == 1 or not args.no_windows),
-                       "prefill_pieces": args.seq_chunks if world > 1 else 1,
+                       "prefill_pieces": args.seq_chunks if world > 1 else 1, "kv_dtype": args.kv_dtype,
                        "decode_windows": getattr(engine, "windows", 0)},
             "decode": {"tokens_per_s": round(dec_tokens / (dec_ms / 1e3), 1), "steps": steps_dec,
                        "ms_per_step": round(step_ms, 3)},
@@ -845,7 +855,7 @@ def profile_case(name: str, reps: int, timed: bool = False):
             graph.replay()
         wbytes = sum(t.numel() * 2 for t in (wqkv, wo, wgu, wd))
         work = (per_replay * wbytes, "B")
-    elif name == "decode_layer":       # one whole decode layer of the C4 batch (8 layers per CUDA graph replay)
+    elif name in ("decode_layer", "decode_layer_e4m3"):   # one whole decode layer of the C4 batch (8 a graph replay)
         import random
         from forgeserve_b200 import ModelConfig
         from forgeserve_b200.model import Block, RopeTables, layer_forward_
@@ -862,9 +872,16 @@ def profile_case(name: str, reps: int, timed: bool = False):
         it = iter(blocks)
         W = max(widths)
         table = torch.tensor([[next(it) for _ in range(w)] + [0] * (W - w) for w in widths], device=dev)
-        pool = PagedKVPool(cfg, nblk, bs, dtype=torch.bfloat16, device=dev, n_layers=1)
-        pool.k[0].normal_(generator=g)
-        pool.v[0].normal_(generator=g)
+        kv_dtype = "e4m3" if name.endswith("e4m3") else "model"
+        pool = PagedKVPool(cfg, nblk, bs, dtype=KV_DTYPES[kv_dtype] or torch.bfloat16, device=dev, n_layers=1)
+        for t in (pool.k[0], pool.v[0]):
+            if pool.quantized:                            # codes and scales of values near 1
+                t.copy_(rnd(*t.shape, scale=150.0).clamp_(-448, 448))
+            else:
+                t.normal_(generator=g)
+        if pool.quantized:
+            pool.k_scale[0].fill_(1 / 150)
+            pool.v_scale[0].fill_(1 / 150)
         blk = Block(cfg, device=dev, dtype=torch.bfloat16)
         with torch.no_grad():
             for pname, prm in blk.named_parameters():
@@ -893,7 +910,7 @@ def profile_case(name: str, reps: int, timed: bool = False):
         def fn():
             graph.replay()
         weight_bytes = sum(prm.numel() * prm.element_size() for prm in blk.parameters())
-        kv_bytes = sum(n + 1 for n in lengths) * nkv * hd * 2 * 2
+        kv_bytes = sum(n + 1 for n in lengths) * nkv * 2 * kv_row_bytes(hd, kv_dtype)
         print(json.dumps({"decode_layer_weight_bytes": weight_bytes, "kv_bytes": kv_bytes, "layers_per_launch": 8}))
         work = (per_replay * (weight_bytes + kv_bytes + 4.0 * rows * d * 2), "B")
     else:
@@ -956,6 +973,8 @@ def main():
     ap.add_argument("--c5-sweep", default="", help="c5: comma-separated micro-batch counts (default 4,8,16,32)")
     ap.add_argument("--microbatches", type=int, default=0, help="c4 with N > 1: micro-batches per engine step")
     ap.add_argument("--no-graphs", action="store_true", help="c4: launch every decode kernel from Python")
+    ap.add_argument("--kv-dtype", choices=list(KV_DTYPES), default="model",
+                    help="c4: the block pool's type (e4m3: the engines' 8-bit pool; not the workload's own precision)")
     ap.add_argument("--no-windows", action="store_true", help="c4 with N > 1: drain the pipeline after every step")
     ap.add_argument("--profile-case", default=None,
                     help="run a few launches of one kernel (for ncu) and exit; a comma-separated list runs several")
