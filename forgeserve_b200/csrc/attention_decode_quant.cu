@@ -306,8 +306,8 @@ struct Geo {
   static constexpr int BOXES = HD / BOX;                      // boxes a row
   static constexpr int STEP_BYTES = STEP * HD;                // K (or V) of a step
   // A warp's ring is one step deep: K of the next step is on its way from the scores on, its V from the V product on.
-  // Two steps take the shared memory of a fourth CTA an SM (64 rows: 89 us against 80), four for CTAs alone on an SM save
-  // 0.3 us of 11.
+  // At hd 128 two steps take the shared memory of a fourth CTA an SM (64 rows: 89 us against 80), four for CTAs alone on
+  // an SM save 0.3 us of 11. Not tried at hd 64, where the issue slots, not the bytes on their way, are short.
   static constexpr int BUF = 2 * STEP_BYTES;                  // a warp's K, then V
   static constexpr int Q_OFF = WARPS * BUF;                   // q as B operands: [NT][PARTS][KS][32 lanes] of 8 bytes
   static constexpr int AT_OFF = Q_OFF + NT * PARTS * KS * 256;   // places: [2][values, scales][WARPS][LOOK]
@@ -318,8 +318,9 @@ struct Geo {
   static constexpr int O_BYTES = WARPS * 8 * NT * (O_ROW + 3) * 4;   // the merge: sums, (max, sum), weights
   static_assert(!WHOLE || O_BYTES <= BAR_OFF, "the merge must leave the barriers alone");
   static constexpr int SMEM = (O_BYTES > END ? O_BYTES : END) + (WHOLE ? 1024 : 0);   // boxes lie on 1024 bytes
-  // CTAs an SM that the registers are held to: the most that spill little (hd 128: 80 us on 64 rows at 4, 87 at 3; 16
-  // heads a KV head 65 at 3, 76 unbounded; hd 64, MHA 50 at 6, 55 at 4; hd 256 31 at 3, 34 unbounded).
+  // CTAs an SM that the registers are held to, measured in bf16 (hd 128: 80 us on 64 rows at 4, 87 at 3; 16 heads a KV head
+  // 65 at 3, 76 unbounded; hd 64, MHA 50 at 6, 55 at 4; hd 256 31 at 3, 34 unbounded). bf16 then spills up to 8 bytes a
+  // thread, 136 at hd 256 with two N tiles; fp32 up to 28, at hd 256 188 with one N tile and 436 with two.
   static constexpr int CTAS = NT == 1 ? (HD == 64 ? (sizeof(T) == 2 ? 6 : 5) : HD == 128 ? 4 : 3)
                                       : (HD == 64 ? 4 : HD == 128 ? 3 : 2);
   // byte of a K (or V) step's 16-byte chunk `chunk` of row `row`

@@ -458,7 +458,8 @@ __global__ void __launch_bounds__(256, CTAS)
 
 // STAGED: a head's values go through shared memory, where its lanes take the pairs in turn (neighbouring ones at a time,
 // so that tables and banks are read in order). 8192 tokens of 32 + 8 + 8 heads of 128, 126 turned: 53 us to the 8-bit
-// cache, 51 to the bf16 one, 69 in fp32, where a warp a head, as above, takes 178, 171 and 197.
+// cache, 51 to the bf16 one, 69 in fp32, where a warp a head, as above, takes 178, 171 and 197. The whole pieces of HALVES
+// take 33 to both: here an item's pieces are loaded when it begins, and nothing is on its way while they turn.
 template <typename T, bool QUANT>
 __global__ void __launch_bounds__(256, WRITE_CTAS)
     rotary_write_staged_kernel(WriteParams p, int lanes, unsigned groups) {

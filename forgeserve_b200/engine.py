@@ -379,8 +379,8 @@ class Engine(Scheduler):
     back, without a host synchronisation per step. A tensor-parallel model (its all-reduces run through
     torch.distributed) always launches eagerly and steps one at a time.
 
-    kv_dtype=torch.float8_e4m3fn (extra): an 8-bit block pool (PagedKVPool), half the cache bytes of bf16, so twice the
-    blocks in the same memory; keys and values are rounded as they are written.
+    kv_dtype=torch.float8_e4m3fn (extra): an 8-bit block pool (PagedKVPool), (head_dim + 4) / (2 head_dim) of the cache
+    bytes of bf16 (0.52 at head_dim 128, 0.53 at 64); keys and values are rounded as they are written.
 
     Under tensor parallelism every shard runs the same Engine over its own model shard (model.tp): the pool holds
     the shard's KV heads, the logits are replicated, so every shard samples the same tokens (engine.py:36-45 with
