@@ -86,6 +86,8 @@ SIGNATURES = {
                                          ctypes.POINTER(KVQuantDesc), c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_int,
                                          c_int, c_vp]),
     "fs_kv_dequant": (c_int, [ctypes.POINTER(KVQuantDesc), c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_vp]),
+    "fs_kv_dequant_for": (c_int, [ctypes.POINTER(KVQuantDesc), c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_int,
+                                  c_vp]),
     "fs_attention_decode_quant_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64]),
     "fs_attention_decode_quant": (c_int, [c_vp, c_i64, ctypes.POINTER(KVQuantDesc), c_i64, c_vp, c_vp, c_i64, c_i64,
                                           c_i64, c_i64, c_i64, c_float, c_vp, c_i64, c_int, c_vp]),

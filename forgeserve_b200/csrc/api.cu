@@ -412,19 +412,31 @@ int fs_rotary_kv_write_quant(const void* qkv, int64_t ld, void* q_out, int64_t l
                        positions, &kv->cache, &sc, B, T, nh, nkv, hd, slot_base, slot_from_pos, dtype, stream);
 }
 
-int fs_kv_dequant(const fs_kv_quant* kv, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd, void* k_out, void* v_out,
-                  int dtype, void* stream) {
+static int dequant_common(const std::string& who, const fs_kv_quant* kv, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd,
+                          const int64_t* positions, int64_t T, void* k_out, void* v_out, int dtype, void* stream) {
   if (B <= 0 || n_slots <= 0) return 0;
   if (check_kv_quant(kv)) return -1;
-  if (!dtype_ok(dtype)) return fail("fs_kv_dequant: unsupported dtype");
-  if (!k_out || !v_out) return fail("fs_kv_dequant: NULL pointer");
-  if (hd <= 0 || nkv <= 0 || hd > 65536) return fail("fs_kv_dequant: bad head_dim or head count");
-  if (B > 65535 || nkv > 65535) return fail("fs_kv_dequant: too many rows or heads");
-  if (n_slots > INT32_MAX || n_slots * hd > INT32_MAX * int64_t(128)) return fail("fs_kv_dequant: too many slots");
+  if (!dtype_ok(dtype)) return fail(who + ": unsupported dtype");
+  if (!k_out || !v_out) return fail(who + ": NULL pointer");
+  if (hd <= 0 || nkv <= 0 || hd > 65536) return fail(who + ": bad head_dim or head count");
+  if (B > 65535 || nkv > 65535) return fail(who + ": too many rows or heads");
+  if (n_slots > INT32_MAX || n_slots * hd > INT32_MAX * int64_t(128)) return fail(who + ": too many slots");
   if ((n_slots - 1) / kv->cache.block_size >= kv->cache.table_cols)
-    return fail("fs_kv_dequant: the block table covers fewer slots");
-  return kv_dequant(dtype, to_internal(&kv->cache), to_scales(kv), B, n_slots, nkv, hd, k_out, v_out,
+    return fail(who + ": the block table covers fewer slots");
+  return kv_dequant(dtype, to_internal(&kv->cache), to_scales(kv), B, n_slots, nkv, hd, positions, T, k_out, v_out,
                     static_cast<cudaStream_t>(stream));
+}
+
+int fs_kv_dequant(const fs_kv_quant* kv, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd, void* k_out, void* v_out,
+                  int dtype, void* stream) {
+  return dequant_common("fs_kv_dequant", kv, B, n_slots, nkv, hd, nullptr, 0, k_out, v_out, dtype, stream);
+}
+
+int fs_kv_dequant_for(const fs_kv_quant* kv, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd, const int64_t* positions,
+                      int64_t T, void* k_out, void* v_out, int dtype, void* stream) {
+  if (B > 0 && n_slots > 0 && (!positions || T <= 0 || T > INT32_MAX))
+    return fail("fs_kv_dequant_for: positions of at least one query a row needed");
+  return dequant_common("fs_kv_dequant_for", kv, B, n_slots, nkv, hd, positions, T, k_out, v_out, dtype, stream);
 }
 
 int64_t fs_attention_decode_quant_workspace(int64_t B, int64_t nh, int64_t nkv, int64_t hd, int64_t n_slots) {

@@ -66,8 +66,9 @@ int rotary_kv_write(int dtype, const void* qkv, int64_t ld, void* q_out, int64_t
                     const float* sin_t, int64_t rope_rows, int64_t rd, int interleaved, const int64_t* positions,
                     const KVCache& kv, const KVScales* sc, int64_t B, int64_t T_new, int64_t nh, int64_t nkv,
                     int64_t hd, int64_t slot_base, int slot_from_pos, cudaStream_t st);
+// positions (B, T), or nullptr: what past their last one a row's table names is not flagged.
 int kv_dequant(int dtype, const KVCache& kv, const KVScales& sc, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd,
-               void* k_out, void* v_out, cudaStream_t st);
+               const int64_t* positions, int64_t T, void* k_out, void* v_out, cudaStream_t st);
 
 namespace decode_quant {   // attention_decode_quant.cu
 int64_t workspace_bytes(int64_t B, int64_t nh, int64_t nkv, int64_t hd, int64_t n_slots);

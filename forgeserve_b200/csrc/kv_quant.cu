@@ -547,6 +547,22 @@ bool write_vec_ok(const WriteParams& p, bool quant) {
   return (all & 15) == 0;
 }
 
+// Flags the bad blocks of a read-back for given queries: those that one of their row's T positions reaches. Table columns
+// that no query looks at may hold anything. One thread a column; only a bad block's looks through the positions. A kernel of
+// its own: the same test inside the read-back cost that one 4 to 9 % by its registers.
+__global__ void __launch_bounds__(256)
+    flag_seen_blocks_kernel(KVCache kv, int64_t cols, const int64_t* __restrict__ positions, int T, unsigned* err) {
+  pdl_trigger();
+  pdl_wait();   // launched with PDL: everything below reads other kernels' data
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x, r = blockIdx.y;
+  if (col >= cols) return;
+  const int64_t blk = kv.table[r * kv.table_stride + col];
+  if (blk >= 0 && blk < kv.num_blocks) return;
+  bool seen = false;
+  for (int t = 0; t < T && !seen; ++t) seen = positions[r * T + t] >= col * kv.block_size;
+  if (seen) flag_error(err, ERR_BAD_SLOT);
+}
+
 // Values of `n_slots` slots of every row, k and v: one thread a value of each.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -688,9 +704,16 @@ int rotary_kv_write(int dtype, const void* qkv, int64_t ld, void* q_out, int64_t
 }
 
 int kv_dequant(int dtype, const KVCache& kv, const KVScales& sc, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd,
-               void* k_out, void* v_out, cudaStream_t st) {
+               const int64_t* positions, int64_t T_new, void* k_out, void* v_out, cudaStream_t st) {
   unsigned* err = error_word();
   if (!err) return -1;
+  if (positions) {
+    const int64_t cols = (n_slots - 1) / kv.block_size + 1;
+    const dim3 grid(static_cast<unsigned>((cols + 255) / 256), static_cast<unsigned>(B));
+    launch_pdl_async(flag_seen_blocks_kernel, grid, 256, 0, st, kv, cols, positions, static_cast<int>(T_new), err);
+    if (check_launch("flag_seen_blocks_kernel")) return -1;
+    err = nullptr;   // the read-back itself reports nothing
+  }
   const int vec = dtype == F32 ? 4 : 8;
   const uintptr_t out = reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out);
   const uintptr_t in = reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v);

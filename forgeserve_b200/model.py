@@ -230,7 +230,7 @@ def layer_forward_(blk: "Block", x: torch.Tensor, positions: torch.Tensor, kv, r
     quant = isinstance(desc, L.KVQuantDesc)
     if quant and T > 1:
         # several new tokens a row over an 8-bit cache: attention over the table's slots read back as dense tensors
-        k_all, v_all = ops.kv_dequant(kv.read_descriptor(), B, n_slots, nkv, hd, x.dtype)
+        k_all, v_all = ops.kv_dequant(desc, B, n_slots, nkv, hd, x.dtype, positions)
         table = row_table(B, x.device)
         desc, keep = ops.contiguous_desc(k_all, v_all, table), (keep, k_all, v_all, table)
     attn = torch.empty(B, T, nh * hd, dtype=x.dtype, device=x.device)

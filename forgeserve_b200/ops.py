@@ -358,8 +358,11 @@ def rotary_kv_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optiona
     return q_out
 
 
-def kv_dequant(kv: L.KVQuantDesc, B: int, n_slots: int, nkv: int, hd: int, dtype: torch.dtype):
-    """The first n_slots slots of every row of an 8-bit cache as dense (k, v), each (B, nkv, n_slots, hd) of dtype."""
+def kv_dequant(kv: L.KVQuantDesc, B: int, n_slots: int, nkv: int, hd: int, dtype: torch.dtype,
+               positions: Optional[torch.Tensor] = None):
+    """The first n_slots slots of every row of an 8-bit cache as dense (k, v), each (B, nkv, n_slots, hd) of dtype. A block
+    number outside the cache reads as zeros and raises the bad slot flag; with positions (B, T), those of the queries that
+    look at the result, only where a row's last one reaches the block."""
     codes = kv.keep[0]
     if not codes.is_cuda:
         require_cuda(codes)
@@ -368,7 +371,16 @@ def kv_dequant(kv: L.KVQuantDesc, B: int, n_slots: int, nkv: int, hd: int, dtype
     _check_quant_cache(kv, B, nkv, hd, dev)
     k = torch.empty((B, nkv, n_slots, hd), dtype=dtype, device=dev)
     v = torch.empty_like(k)
-    _run("fs_kv_dequant", L.load().fs_kv_dequant, dev, kv, B, n_slots, nkv, hd, k.data_ptr(), v.data_ptr(), code)
+    if positions is None:
+        _run("fs_kv_dequant", L.load().fs_kv_dequant, dev, kv, B, n_slots, nkv, hd, k.data_ptr(), v.data_ptr(), code)
+    elif positions.numel():
+        T = positions.shape[-1]
+        _check_positions(positions, B * T)
+        _on_device(dev, positions)
+        _run("fs_kv_dequant_for", L.load().fs_kv_dequant_for, dev, kv, B, n_slots, nkv, hd, positions.data_ptr(), T,
+             k.data_ptr(), v.data_ptr(), code)
+    else:
+        raise ValueError("kv_dequant: positions of at least one query a row needed")
     return k, v
 
 

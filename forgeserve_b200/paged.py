@@ -74,23 +74,14 @@ class PagedKVPool:
         dev = self.device
         tables = torch.as_tensor(block_tables).to(device=dev, dtype=torch.int64, non_blocking=True).contiguous()
         pos = torch.as_tensor(positions).to(device=dev, dtype=torch.int64, non_blocking=True).contiguous()
-        seen = seen_tables(tables, pos, self.block_size) if self.quantized and pos.shape[1] > 1 else None
-        return [PagedLayerView(self, layer, tables, pos, seen) for layer in range(len(self.k))]
-
-
-def seen_tables(tables: torch.Tensor, positions: torch.Tensor, block_size: int) -> torch.Tensor:
-    """tables with block 0 in the columns past each row's last position, which may hold anything."""
-    cols = torch.arange(tables.shape[1], device=tables.device)
-    return torch.where(cols <= positions.amax(1, keepdim=True) // block_size, tables, 0)
+        return [PagedLayerView(self, layer, tables, pos) for layer in range(len(self.k))]
 
 
 class PagedLayerView:
     """What one attention layer sees during one step (same interface as ContiguousKV.update)."""
 
-    def __init__(self, pool: PagedKVPool, layer: int, block_tables: torch.Tensor, positions: torch.Tensor,
-                 seen: Optional[torch.Tensor] = None):
+    def __init__(self, pool: PagedKVPool, layer: int, block_tables: torch.Tensor, positions: torch.Tensor):
         self.pool, self.layer, self.tables, self.positions = pool, layer, block_tables, positions
-        self._seen = seen    # seen_tables of this step, which its layers share
 
     @property
     def length(self) -> int:
@@ -102,19 +93,9 @@ class PagedLayerView:
 
     def descriptor(self):
         if self.pool.quantized:
-            return self._quant_descriptor(self.tables)
+            return ops.quant_paged_desc(self.pool.k[self.layer], self.pool.v[self.layer],
+                                        self.pool.k_scale[self.layer], self.pool.v_scale[self.layer], self.tables)
         return ops.paged_desc(self.pool.k[self.layer], self.pool.v[self.layer], self.tables)
-
-    def _quant_descriptor(self, tables: torch.Tensor):
-        return ops.quant_paged_desc(self.pool.k[self.layer], self.pool.v[self.layer], self.pool.k_scale[self.layer],
-                                    self.pool.v_scale[self.layer], tables)
-
-    def read_descriptor(self):
-        """Descriptor of an 8-bit pool for reading back all n_slots of every row: block 0 stands for what lies past a
-        row's last position."""
-        if self._seen is None:
-            self._seen = seen_tables(self.tables, self.positions, self.pool.block_size)
-        return self._quant_descriptor(self._seen)
 
     def update(self, k: torch.Tensor, v: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """Store k, v (B, n_kv, T, head_dim) at their positions; return each row's blocks in table order as

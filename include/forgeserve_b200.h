@@ -210,6 +210,11 @@ int fs_rotary_kv_write_quant(const void* qkv, int64_t ld, void* q_out, int64_t l
 int fs_kv_dequant(const fs_kv_quant* kv, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd, void* k_out, void* v_out,
                   int dtype, void* stream);
 
+/* fs_kv_dequant for attention of T queries a row at positions (B, T): a block number outside the cache whose slots lie past
+ * the row's last position, where no query looks, still reads as zeros but flags nothing. */
+int fs_kv_dequant_for(const fs_kv_quant* kv, int64_t B, int64_t n_slots, int64_t nkv, int64_t hd, const int64_t* positions,
+                      int64_t T, void* k_out, void* v_out, int dtype, void* stream);
+
 /* fs_attention_decode over an 8-bit cache: one query a row, any n_heads / n_kv_heads, head_dim even and <= 256. A row
  * with a negative position sees no slot and gets zeros. workspace: fs_attention_decode_quant_workspace(...) bytes (0 up
  * to 512 slots), 16-byte aligned, as for fs_attention_decode. */

@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 
 from forgeserve_b200 import _lib as L
 from forgeserve_b200 import Engine, ForgeModel, ModelConfig, PagedKVPool, generate, ops
-from forgeserve_b200.model import _rope_write, rope_tables
+from forgeserve_b200.model import _rope_write, layer_forward_, rope_tables
 from oracle import forge_oracle as O
 
 DEV = "cuda"
@@ -1196,3 +1196,82 @@ def test_tables_padded_with_no_block(kind, dtype, hd):
         got.append(torch.cat(logits, 1))
         assert L.device_error() == 0, pad
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+@pytest.mark.parametrize("dtype", [F8, torch.float32])
+def test_tables_of_more_rows_than_the_step(dtype):
+    """A step takes the first rows of a table that has more; one of fewer rows is refused over an 8-bit pool."""
+    cfg, m = model_pair(torch.float32)
+    idx = torch.randint(0, 64, (2, 9), generator=torch.Generator().manual_seed(1))
+    pos = torch.arange(9).expand(2, 9)
+    table = torch.arange(15).view(5, 3)
+    got = []
+    for t in (table, table[:2]):
+        pool = PagedKVPool(cfg, 16, 4, dtype=dtype, device=DEV)
+        a = m(idx[:, :8], pos[:, :8], pool.views(t, pos[:, :8]))
+        got.append(torch.cat([a, m(idx[:, 8:], pos[:, 8:], pool.views(t, pos[:, 8:]))], 1))
+    assert torch.equal(*got)
+    if dtype == F8:
+        with pytest.raises(ValueError, match="rows"):
+            m(idx, pos, pool.views(table[:1], pos))
+
+
+@pytest.mark.parametrize("hd", [128, 18])
+def test_dequant_for_queries_flags_what_they_see(hd):
+    """Bad blocks: of a row that no query sees, of rows whose first, middle or last query reaches them, or ends one slot
+    before."""
+    bs, T = 4, 3
+    k, v, ks, vs = quant_pool(6, 2, bs, hd, 9)
+    table = torch.tensor([[1, -1, 99, 2], [3, 4, 5, -7]], device=DEV)
+    desc = ops.quant_paged_desc(k, v, ks, vs, table)
+    plain, _ = ops.kv_dequant(desc, 2, 16, 2, hd, torch.float32)
+    assert L.device_error(clear=True) == L.FS_ERR_BAD_SLOT
+    for pos, bad in (([[0, 1, 3], [9, 10, 11]], False), ([[0, 1, 4], [0, 0, 0]], True), ([[4, 1, 0], [0, 0, 0]], True),
+                     ([[-1, -1, -1], [0, 12, 3]], True), ([[-1, 3, -1], [11, 0, 0]], False),
+                     ([[0, 0, 0], [0, 0, 1000]], True)):
+        kd, vd = ops.kv_dequant(desc, 2, 16, 2, hd, torch.float32, torch.tensor(pos, device=DEV))
+        assert L.device_error(clear=True) == (L.FS_ERR_BAD_SLOT if bad else 0), pos
+        assert torch.equal(kd, plain) and not vd[0, :, 4:12].any() and not vd[1, :, 12:].any()
+    for pos in (torch.zeros(2, 0, dtype=torch.int64, device=DEV), torch.zeros(3, 2, dtype=torch.int64, device=DEV),
+                torch.zeros(2, 3, device=DEV)):
+        with pytest.raises(ValueError, match="positions"):
+            ops.kv_dequant(desc, 2, 16, 2, hd, torch.float32, pos)
+
+
+@torch.no_grad()
+def test_captured_chunk_over_an_8bit_pool():
+    """A step of several tokens captured once over views of static tables and positions, replayed as both move on."""
+    cfg, m = model_pair(torch.float32)
+    idx = torch.randint(0, 64, (1, 40), generator=torch.Generator().manual_seed(1)).to(DEV)
+    pos = torch.arange(40, device=DEV)[None]
+    blocks = torch.randperm(12, generator=torch.Generator().manual_seed(2))[:10].to(DEV)
+    want_pool, pool = (PagedKVPool(cfg, 12, 4, dtype=F8, device=DEV) for _ in range(2))
+    cos, sin = m._rope.on(torch.device(DEV))
+
+    def step(tokens, positions, views):
+        x = ops.embed(tokens, m.tok_emb.weight)
+        for blk, view in zip(m.layers, views):
+            layer_forward_(blk, x, positions, view, cos, sin)
+        return x
+
+    cuts = [slice(a, a + 4) for a in range(0, 40, 4)]
+    want = [step(idx[:, c], pos[:, c].contiguous(), want_pool.views(blocks[None], pos[:, c])) for c in cuts]
+    toks, p, table = idx[:, :4].clone(), pos[:, :4].clone(), torch.full((1, 10), -1, device=DEV)
+    table[0, 0] = blocks[0]
+    views = pool.views(table, p)
+    assert views[0].tables.data_ptr() == table.data_ptr() and views[0].positions.data_ptr() == p.data_ptr()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        step(toks, p, views)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        out = step(toks, p, views)
+    for i, c in enumerate(cuts):
+        toks.copy_(idx[:, c])
+        p.copy_(pos[:, c])
+        table[0, i] = blocks[i]
+        g.replay()
+        assert torch.equal(out, want[i]), i
+    assert torch.equal(bits(pool.k[1][blocks]), bits(want_pool.k[1][blocks]))

@@ -229,3 +229,16 @@ def test_config_refuses_rotary_dims_that_are_no_whole_numbers():
     for bad in (8.0, "8", True):
         with pytest.raises(ValueError, match="rotary_dim"):
             ModelConfig(rotary_dim=bad)
+
+
+def test_dequant_for_queries_refusals(lib):
+    d = quant_desc()
+
+    def deq(kv=ctypes.byref(d), B=1, n=16, pos=P, T=3, k=P, v=P, dtype=L.FS_BF16):
+        return lib.fs_kv_dequant_for(kv, B, n, 2, 128, pos, T, k, v, dtype, None)
+
+    for kw, word in ((dict(pos=None), b"positions"), (dict(T=0), b"positions"), (dict(T=-1), b"positions"),
+                     (dict(T=1 << 31), b"positions"), (dict(kv=None), b"descriptor"), (dict(v=None), b"NULL"),
+                     (dict(dtype=5), b"dtype"), (dict(n=129), b"fewer slots"), (dict(B=70000), b"too many")):
+        assert deq(**kw) == -1 and word in lib.fs_last_error(), (kw, lib.fs_last_error())
+    assert deq(n=0, pos=None) == 0 and deq(B=0, T=0) == 0
